@@ -36,6 +36,7 @@
 #include "tcw.h"
 #include "tessera_b200.h"
 #include "tessera_b200_ops.h"
+#include "token_ops.h"
 
 namespace tcb {
 
@@ -1062,6 +1063,67 @@ int tcb_op_out128(const void *r2, int64_t P, const uint8_t *empty, float *out, i
                   void *stream) {
     OP_TRY("tcb_op_out128", launch_out128(static_cast<const bf16 *>(r2), P, empty, out, codes, scales,
                                           static_cast<cudaStream_t>(stream)))
+}
+
+int tcb_op_rmsnorm(const void *x, int64_t ldx, const void *res, int64_t ldr, void *sum, int64_t lds, const float *g,
+                   float eps, int dtype, void *y, int64_t ldy, int ytype, float *scales, int group, int64_t M, int D,
+                   void *stream) {
+    OP_TRY("tcb_op_rmsnorm", {
+        RmsArgs a;
+        a.x = x; a.ldx = ldx; a.res = res; a.ldr = ldr; a.sum = sum; a.lds = lds;
+        a.g = g; a.eps = eps; a.y = y; a.ldy = ldy; a.scales = scales; a.group = group;
+        a.M = M; a.D = D;
+        launch_rmsnorm(a, dtype, ytype, static_cast<cudaStream_t>(stream));
+    })
+}
+
+int tcb_op_rope(const void *x, int64_t ldx, int64_t hsx, int dtype, const void *pos, int64_t pos_stride, int pos_type,
+                const double *freq, float mscale, int rot, int interleaved, int inverse, void *out, int64_t ldo,
+                int64_t hso, int64_t M, int heads, int hd, void *stream) {
+    OP_TRY("tcb_op_rope", {
+        RopeArgs a;
+        a.x = x; a.ldx = ldx; a.hsx = hsx; a.pos = pos; a.pos_stride = pos_stride; a.freq = freq;
+        a.mscale = mscale; a.sign = inverse ? -1.f : 1.f; a.rot = rot;
+        a.out = out; a.ldo = ldo; a.hso = hso; a.M = M; a.heads = heads; a.hd = hd;
+        launch_rope(a, dtype, pos_type, interleaved != 0, static_cast<cudaStream_t>(stream));
+    })
+}
+
+int tcb_op_gemv_w4(const void *x, int64_t ldx, int xtype, const float *xscales, int xgroup, const void *w, int group,
+                   const float *bias, int relu, const void *res, int64_t ldr, void *out, int64_t ldo, int otype, int M,
+                   int N, int K, void *stream) {
+    OP_TRY("tcb_op_gemv_w4", {
+        W4Args a;
+        a.x = x; a.ldx = ldx; a.xscales = xscales; a.xgroup = xgroup; a.w = w; a.group = group;
+        a.bias = bias; a.relu = relu; a.res = res; a.ldr = ldr; a.out = out; a.ldo = ldo;
+        a.M = M; a.N = N; a.K = K;
+        launch_gemv_w4(a, xtype, otype, static_cast<cudaStream_t>(stream));
+    })
+}
+
+// Host helpers: as OP_TRY, without a CUDA call.
+#define HOST_TRY(name, body)                                                                       \
+    try {                                                                                          \
+        body;                                                                                      \
+        return 0;                                                                                  \
+    } catch (const std::exception &e) {                                                            \
+        std::fprintf(stderr, "%s: %s\n", name, e.what());                                          \
+        return -1;                                                                                 \
+    }
+
+int tcb_rope_freqs(int rot, double base, int scaling, double factor, double span, double fast, double slow, double *freq,
+                   float *mscale) {
+    HOST_TRY("tcb_rope_freqs", rope_freqs(rot, base, scaling, factor, span, fast, slow, freq, mscale))
+}
+
+int64_t tcb_w4_bytes(int N, int K, int group) { return w4_bytes(N, K, group); }
+
+int tcb_w4_pack(const float *w, int N, int K, int group, void *packed) {
+    HOST_TRY("tcb_w4_pack", w4_pack(w, N, K, group, packed))
+}
+
+int tcb_w4_pack_codes(const int8_t *codes, const float *scales, int N, int K, int group, void *packed) {
+    HOST_TRY("tcb_w4_pack_codes", w4_pack_codes(codes, scales, N, K, group, packed))
 }
 
 int tcb_attention_plan(const int64_t *off, int64_t npix, int32_t *list, int64_t *n, int32_t *tmax) {

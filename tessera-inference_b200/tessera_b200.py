@@ -24,7 +24,13 @@ EXPORTED = [
     "tc_host_free",
     "tcb_op_gemm", "tcb_op_gemm_ln", "tcb_op_gemm_ln_noalloc", "tcb_op_count", "tcb_op_gather", "tcb_op_emb1", "tcb_op_attention",
     "tcb_op_layernorm640", "tcb_op_pool", "tcb_op_ln_relu2560", "tcb_op_out128", "tcb_op_wait_probe", "tcb_attention_plan",
+    "tcb_op_rmsnorm", "tcb_op_rope", "tcb_rope_freqs", "tcb_op_gemv_w4", "tcb_w4_bytes", "tcb_w4_pack",
+    "tcb_w4_pack_codes",
 ]
+
+# element types of the token-stream operators (TCB_* in include/tessera_b200_ops.h)
+BF16, F16, F32, I8, E4M3, I32, I64 = range(7)
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_WAVES = range(4)
 
 CAT_NAMES = ["h2d", "prep", "emb1", "gemm", "attention", "layernorm", "pool", "head", "d2h"]
 GEMM_KINDS = ["emb2", "qkv", "out", "ffn1", "ffn2", "head"]
@@ -115,6 +121,21 @@ def load_library(path: os.PathLike | None = None) -> C.CDLL:
     lib.tcb_op_wait_probe.argtypes = [i64, vp, vp]
     lib.tcb_attention_plan.restype = i32
     lib.tcb_attention_plan.argtypes = [vp, i64, vp, vp, vp]
+    lib.tcb_op_rmsnorm.restype = i32
+    lib.tcb_op_rmsnorm.argtypes = [vp, i64, vp, i64, vp, i64, vp, C.c_float, i32, vp, i64, i32, vp, i32, i64, i32, vp]
+    lib.tcb_op_rope.restype = i32
+    lib.tcb_op_rope.argtypes = [vp, i64, i64, i32, vp, i64, i32, vp, C.c_float, i32, i32, i32, vp, i64, i64, i64, i32,
+                                i32, vp]
+    lib.tcb_rope_freqs.restype = i32
+    lib.tcb_rope_freqs.argtypes = [i32, C.c_double, i32] + [C.c_double] * 4 + [vp, C.POINTER(C.c_float)]
+    lib.tcb_op_gemv_w4.restype = i32
+    lib.tcb_op_gemv_w4.argtypes = [vp, i64, i32, vp, i32, vp, i32, vp, i32, vp, i64, vp, i64, i32, i32, i32, i32, vp]
+    lib.tcb_w4_bytes.restype = i64
+    lib.tcb_w4_bytes.argtypes = [i32, i32, i32]
+    lib.tcb_w4_pack.restype = i32
+    lib.tcb_w4_pack.argtypes = [vp, i32, i32, i32, vp]
+    lib.tcb_w4_pack_codes.restype = i32
+    lib.tcb_w4_pack_codes.argtypes = [vp, vp, i32, i32, i32, vp]
     lib.tcb_op_out128.restype = i32
     lib.tcb_op_out128.argtypes = [vp, i64, vp, vp, vp, vp, vp]
     if path is None:
@@ -228,6 +249,38 @@ def attention_plan(off: np.ndarray) -> tuple[list[np.ndarray], list[int]]:
         raise RuntimeError("tcb_attention_plan failed")
     b = np.concatenate([[0], np.cumsum(n)])
     return [lst[b[c]:b[c + 1]].copy() for c in range(3)], [int(t) for t in tmax]
+
+
+def rope_freqs(rot: int, base: float = 10000.0, scaling: int = ROPE_PLAIN, factor: float = 1.0, span: float = 0.0,
+               fast: float = 32.0, slow: float = 1.0) -> tuple[np.ndarray, float]:
+    """tcb_rope_freqs: (rot/2 f64 radians per position, mscale) of tcb_op_rope."""
+    freq = np.zeros(max(rot, 0) // 2, np.float64)
+    m = C.c_float()
+    if load_library().tcb_rope_freqs(rot, base, scaling, factor, span, fast, slow, _ptr(freq), C.byref(m)) != 0:
+        raise RuntimeError("tcb_rope_freqs failed")
+    return freq, m.value
+
+
+def w4_pack(w: np.ndarray, group: int, scales: np.ndarray | None = None) -> np.ndarray:
+    """The packed 4-bit form of a weight matrix (N, K): tcb_w4_pack of f32
+    weights, or tcb_w4_pack_codes of int8 codes in -8..7 with their scales."""
+    lib = load_library()
+    w = np.ascontiguousarray(w, np.float32 if scales is None else np.int8)
+    N, K = w.shape
+    n = lib.tcb_w4_bytes(N, K, group)
+    if n < 0:
+        raise RuntimeError("tcb_w4_bytes failed")
+    out = np.zeros(n, np.uint8)
+    if scales is None:
+        rc = lib.tcb_w4_pack(_ptr(w), N, K, group, _ptr(out))
+    else:
+        scales = np.ascontiguousarray(scales, np.float32)
+        if scales.shape != (N, -(-K // group)):
+            raise ValueError(f"scales of shape {scales.shape}, expected {(N, -(-K // group))}")
+        rc = lib.tcb_w4_pack_codes(_ptr(w), _ptr(scales), N, K, group, _ptr(out))
+    if rc != 0:
+        raise RuntimeError("tcb_w4_pack failed")
+    return out
 
 
 def plan_rows(tile: dict, nparts: int) -> list[int]:

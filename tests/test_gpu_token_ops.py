@@ -1,0 +1,524 @@
+"""The token-stream operators against their definitions in 64 bits.
+
+Tolerances, derived for each output (H = half a step of its type relative to
+the value: bf16 2^-8, fp16 2^-11, f32 2^-24, e4m3 2^-4; an expectation that is
+rounded too costs a second H; U = 2^-24, one f32 rounding):
+
+* RMS norm. A row's squares are summed by threads of at most 64 terms each and
+  a tree of at most 14 levels, all non-negative: (64 + 14 + 1) U. The root
+  halves it; the root, two divisions and three products add 6 U: v is within
+  46 U, taken as 64 U. Codes: v / s is within 130 U of its value, at most 127
+  (448): 0.5 + 127 * 130 U < 0.5 + 1e-3 from the code (e4m3: H of it, or half
+  the smallest step, 2^-10, and 130 U of it).
+* Rotary positions. The fraction of a turn is held to 2^-26 turns, an angle of
+  2 pi 2^-26 < 2 U; sine and cosine are within 4 U; mscale, product and sum add
+  3 U: (|a| + |b|) |mscale| 10 U, plus H of the result.
+* 4-bit product. Every product of a code, at most 8, and an x of at most 11
+  bits is exact in f32. A sum in any order of n = K terms with one extra
+  rounding per group and scale is within (K + 2 K / 32 + 16) U of the sum of
+  magnitudes in the worst case; the matrix instruction may truncate where it
+  adds, which doubles U. The magnitudes are summed in the test.
+"""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import tessera_b200 as tb  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TYPE = {tb.BF16: torch.bfloat16, tb.F16: torch.float16, tb.F32: torch.float32, tb.I8: torch.int8,
+        tb.E4M3: torch.float8_e4m3fn, tb.I32: torch.int32, tb.I64: torch.int64}
+HALF = {tb.BF16: 2.0 ** -8, tb.F16: 2.0 ** -11, tb.F32: 2.0 ** -24}
+TINY = {tb.BF16: 2.0 ** -133, tb.F16: 2.0 ** -24, tb.F32: 2.0 ** -149}  # smallest subnormal
+TOP = {tb.I8: 127.0, tb.E4M3: 448.0}
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return tb.load_library()
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(g, *n):
+    return torch.randn(*n, device="cuda", generator=g)
+
+
+def within(got, want, tol):
+    got, want = got.double(), want.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    fine = ~torch.isnan(want) & (got != want)  # equal infinities are equal
+    err = (got - want).abs()
+    bad = fine & ~(err <= tol)
+    assert not bad.any(), f"{bad.sum().item()} of {bad.numel()} out of tolerance; worst {(err - tol)[bad].max().item()}"
+
+
+# ------------------------------------------------------------------ RMS norm
+def rms_ref(x, res, g, eps):
+    """(h, v) in the definition: h rounded to x's type, v in f64."""
+    h = x if res is None else (x.double() + res.double()).to(x.dtype)
+    d = h.double()
+    v = d / torch.sqrt((d * d).mean(1, keepdim=True) + eps)
+    return h, v if g is None else v * g.double()
+
+
+def check_rms(h, v, y, ytype, group, scales):
+    M, D = v.shape
+    if ytype not in TOP:
+        return within(y, v.to(TYPE[ytype]), v.abs() * (HALF[ytype] * 2 + 64 * U) + TINY[ytype])
+    G = group or D
+    for k, c in enumerate(range(0, D, G)):
+        part, code = v[:, c:c + G], y[:, c:c + G].double()
+        amax = part.abs().amax(1)
+        s = torch.where(torch.isnan(amax), amax, amax.clamp(min=1e-12)) / TOP[ytype]
+        within(scales[:, k], s, s * 80 * U)
+        q = part / s[:, None]
+        if ytype == tb.I8:
+            assert not code[torch.isnan(q)].any()
+            within(torch.where(torch.isnan(q), q, code), q, 0.5 + 1e-3)
+        else:
+            within(code, q, q.abs() * (2.0 ** -4 + 130 * U) + 2.0 ** -10)
+    assert scales.shape[1] == -(-D // G)
+
+
+def run_rms(lib, x, res, g, D, dtype, ytype, group, eps=1e-6, pad=0, want_sum=True, ldy=None):
+    """One call on rows of pitch D + pad; checks that nothing between the rows or behind them is written."""
+    M, ld = x.shape[0], D + pad
+    ldy = ldy or ld
+    y = torch.full((M + 1, ldy), 77, device="cuda").to(TYPE[ytype])
+    sm = torch.full((M + 1, ld), 77, device="cuda").to(TYPE[dtype]) if res is not None and want_sum else None
+    ng = -(-D // group) if group else 1
+    sc = torch.full((M + 1, ng), 77.0, device="cuda") if ytype in TOP else None
+    assert lib.tcb_op_rmsnorm(_p(x), x.stride(0), _p(res), res.stride(0) if res is not None else 0, _p(sm), ld, _p(g), eps,
+                              dtype, _p(y), ldy, ytype, _p(sc), group, M, D, _stream()) == 0
+    torch.cuda.synchronize()
+    mark = torch.tensor([77.0]).to(TYPE[ytype]).float().item()
+    assert (y[M].float() == mark).all() and (y[:, D:].float() == mark).all()
+    if sm is not None:
+        assert (sm[M] == 77).all() and (sm[:, D:] == 77).all()
+        sm = sm[:M, :D]
+    if sc is not None:
+        assert (sc[M] == 77).all()
+        sc = sc[:M]
+    return y[:M, :D], sm, sc
+
+
+def rms_case(lib, M, D, pad, dtype, ytype, group, res, gamma=True, seed=0):
+    g = _gen(seed + M * 7 + D)
+    x = (_randn(g, M, D + pad) * torch.exp(_randn(g, M, 1))).to(TYPE[dtype])
+    r = _randn(g, M, D + pad).to(TYPE[dtype]) if res else None
+    w = 1 + 0.2 * _randn(g, D) if gamma else None
+    if M > 2:
+        x[M // 2] = 0
+        if res:
+            r[M // 2] = 0
+    y, sm, sc = run_rms(lib, x, r, w, D, dtype, ytype, group, pad=pad)
+    h, v = rms_ref(x[:, :D], None if r is None else r[:, :D], w, 1e-6)
+    if res:
+        assert torch.equal(sm, h)
+    check_rms(h, v, y, ytype, group, sc)
+    if M > 2 and ytype in TOP:  # a row of zeros
+        assert not y[M // 2].float().any() and (sc[M // 2] == np.float32(1e-12) / np.float32(TOP[ytype])).all()
+
+
+SIZES = [(1, 1), (3, 2), (5, 7), (4, 31), (4, 32), (7, 33), (9, 96), (3, 127), (33, 128), (5, 200), (130, 640), (7, 641),
+         (6, 1000), (5, 1024), (3, 1032), (5, 1337), (4, 2048), (3, 2560), (2, 4096), (2, 4104), (2, 8191), (2, 8192),
+         (2, 16383), (1, 16384)]
+
+
+@pytest.mark.parametrize("M,D", SIZES)
+@pytest.mark.parametrize("dtype", [tb.BF16, tb.F16, tb.F32])
+def test_rmsnorm_same_type(lib, M, D, dtype):
+    rms_case(lib, M, D, 0, dtype, dtype, 0, True)
+    rms_case(lib, M, D, 5, dtype, dtype, 0, False, gamma=False)
+
+
+@pytest.mark.parametrize("M,D", SIZES)
+@pytest.mark.parametrize("ytype", [tb.I8, tb.E4M3])
+@pytest.mark.parametrize("group", [0, 32, 64, 128])
+def test_rmsnorm_codes(lib, M, D, ytype, group):
+    rms_case(lib, M, D, 0, tb.BF16, ytype, group, True)
+    rms_case(lib, M, D, 3, tb.F16, ytype, group, False)
+    rms_case(lib, M, D, 8, tb.F32, ytype, group, True, gamma=False)
+
+
+def test_rmsnorm_long(lib):
+    """More rows than any grid holds at once."""
+    rms_case(lib, 70001, 640, 0, tb.BF16, tb.E4M3, 128, True)
+    rms_case(lib, 40003, 88, 0, tb.F16, tb.I8, 32, True)
+
+
+@pytest.mark.parametrize("D", [640, 641, 2560, 5001])
+@pytest.mark.parametrize("ytype", [tb.BF16, tb.I8, tb.E4M3])
+def test_rmsnorm_far_values(lib, D, ytype):
+    """Rows whose squares overflow f32, NaN and infinities, and rows that eps alone holds up."""
+    g = _gen(3)
+    x = _randn(g, 6, D)
+    x[0] *= 1e37
+    x[1] *= 1e-30
+    x[2, D // 2] = float("nan")
+    x[3, 1] = float("inf")
+    x[4, D - 1] = float("-inf")
+    x = x.to(torch.bfloat16)
+    group = 0 if ytype == tb.BF16 else 64
+    y, _, sc = run_rms(lib, x, None, None, D, tb.BF16, ytype, group)
+    d = x.double()
+    v = d / torch.sqrt((d * d).mean(1, keepdim=True) + 1e-6)
+    v[1] = d[1] * 1e3  # sqrt(1e-6 + 1e-60) in f32 and f64 alike
+    check_rms(None, v, y, ytype, group, sc)
+
+
+@pytest.mark.parametrize("D,dtype", [(640, tb.BF16), (1337, tb.F16), (2560, tb.F32)])
+def test_rmsnorm_in_place(lib, D, dtype):
+    """sum may be x or res, y may be x or sum."""
+    g = _gen(4)
+    x0, r0 = _randn(g, 50, D).to(TYPE[dtype]), _randn(g, 50, D).to(TYPE[dtype])
+    h, v = rms_ref(x0, r0, None, 1e-5)
+    for which in ("sum=x", "sum=res", "y=x", "y=sum"):
+        x, r, s, y = x0.clone(), r0.clone(), torch.empty_like(x0), torch.empty_like(x0)
+        s = x if which == "sum=x" else r if which == "sum=res" else s
+        y = x if which == "y=x" else s if which == "y=sum" else y
+        assert lib.tcb_op_rmsnorm(_p(x), D, _p(r), D, None if which == "y=sum" else _p(s), D, None, 1e-5, dtype, _p(y), D,
+                                  dtype, None, 0, 50, D, _stream()) == 0
+        check_rms(h, v, y, dtype, 0, None)
+        if which != "y=sum":
+            assert torch.equal(s, h) or which == "y=x" and torch.equal(s, h)
+
+
+def test_rmsnorm_far_pitch(lib):
+    """Row offsets beyond 2^31 elements."""
+    D, ld = 640, 1_300_000_003
+    buf = torch.empty(2 * ld + D, dtype=torch.bfloat16, device="cuda")
+    x = buf.as_strided((3, D), (ld, 1))
+    x.copy_(_randn(_gen(5), 3, D))
+    y, _, sc = run_rms(lib, x, None, None, D, tb.BF16, tb.E4M3, 0)
+    h, v = rms_ref(x, None, None, 1e-6)
+    check_rms(h, v, y, tb.E4M3, 0, sc)
+
+
+# ------------------------------------------------------------------ rotary positions
+def rope_ref(x, pos, freq, mscale, rot, inter, inverse):
+    """x: (M, heads, hd) f64; returns (out, magnitude of the two terms) in f64."""
+    a = pos.double()[:, None] * freq[None]
+    c, s = (a.cos() * mscale)[:, None], (a.sin() * mscale * (-1 if inverse else 1))[:, None]
+    i = torch.arange(rot // 2, device=x.device)
+    p, q = (2 * i, 2 * i + 1) if inter else (i, i + rot // 2)
+    out, mag = x.clone(), torch.zeros_like(x)
+    out[..., p] = x[..., p] * c - x[..., q] * s
+    out[..., q] = x[..., p] * s + x[..., q] * c
+    mag[..., p] = mag[..., q] = (x[..., p].abs() + x[..., q].abs()) * abs(mscale)
+    return out, mag
+
+
+def rope_case(lib, M, heads, hd, rot, dtype, inter, inverse, pos_type=tb.F32, pos_stride=1, gap=0, hgap=0, span=366,
+              mscale=1.0, planes=False, in_place=False, seed=0):
+    """planes: heads outside, rows inside (head stride > row pitch)."""
+    g = _gen(seed + M + 31 * hd + rot)
+    hs = hd + hgap
+    ld = heads * hs + gap
+    if planes:
+        ld, hs = hd + hgap, M * (hd + hgap) + gap
+    n = (M - 1) * ld + (heads - 1) * hs + hd
+    flat = _randn(g, n).to(TYPE[dtype])
+    x = flat.as_strided((M, heads, hd), (ld, hs, 1))
+    pos = torch.randint(0, span, (M, max(pos_stride, 1)), device="cuda", generator=g).to(TYPE[pos_type])
+    p = pos[:, 0] if pos_stride else pos[:1, 0].expand(M)
+    freq = torch.from_numpy(tb.rope_freqs(rot)[0]).cuda()
+    want, mag = rope_ref(x.double(), p, freq, mscale, rot, inter, inverse)
+    oflat = flat if in_place else torch.full((n,), 77.0, device="cuda").to(TYPE[dtype])
+    before = oflat.clone()
+    assert lib.tcb_op_rope(_p(flat), ld, hs, dtype, _p(pos), pos_stride, pos_type, _p(freq), mscale, rot, int(inter),
+                           int(inverse), _p(oflat), ld, hs, M, heads, hd, _stream()) == 0
+    torch.cuda.synchronize()
+    out = oflat.as_strided((M, heads, hd), (ld, hs, 1))
+    within(out, want.to(TYPE[dtype]), mag * 10 * U + want.abs() * 2 * HALF[dtype] + TINY[dtype])
+    assert torch.equal(out[..., rot:].double(), want[..., rot:])
+    out.copy_(before.as_strided(out.shape, out.stride()))
+    assert torch.equal(oflat, before)  # nothing between the heads or rows was written
+
+
+@pytest.mark.parametrize("dtype", [tb.BF16, tb.F16, tb.F32])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("M,heads,hd,rot", [(1, 1, 2, 2), (1, 8, 160, 160), (40, 8, 160, 160), (13, 3, 128, 64), (7, 5, 51, 26),
+                                            (130, 10, 64, 16), (33, 2, 96, 90), (5, 1, 1024, 1024), (3, 48, 256, 130),
+                                            (2, 3, 24, 8), (1000, 1, 16, 16)])
+def test_rope(lib, M, heads, hd, rot, dtype, inter):
+    rope_case(lib, M, heads, hd, rot, dtype, inter, False)
+    rope_case(lib, M, heads, hd, rot, dtype, inter, True, mscale=1.25, gap=hd, hgap=8)
+    rope_case(lib, M, heads, hd, rot, dtype, inter, False, in_place=True, gap=3, hgap=1)
+
+
+@pytest.mark.parametrize("pos_type,stride", [(tb.F32, 1), (tb.F32, 3), (tb.F32, 11), (tb.F32, 0), (tb.I32, 1), (tb.I32, 2),
+                                             (tb.I64, 1), (tb.I64, 0)])
+def test_rope_positions(lib, pos_type, stride):
+    rope_case(lib, 77, 4, 64, 64, tb.F32, False, False, pos_type=pos_type, pos_stride=stride, span=4_000_000)
+    rope_case(lib, 77, 4, 64, 48, tb.BF16, True, False, pos_type=pos_type, pos_stride=stride, span=4_000_000)
+
+
+@pytest.mark.parametrize("dtype", [tb.BF16, tb.F32])
+def test_rope_head_planes(lib, dtype):
+    """Heads outside the rows: (head, row, column) order, aligned and not."""
+    rope_case(lib, 60, 6, 64, 64, dtype, False, False, planes=True)
+    rope_case(lib, 61, 5, 66, 32, dtype, True, False, planes=True, gap=5, hgap=1)
+
+
+def test_rope_far_positions(lib):
+    """Positions past 2^32: the angle keeps its phase. f64 holds pos * freq to 2^-53 of it: 2^40 rad to 2^-13 rad on both
+    sides, so positions stay below 2^33, where both agree to 2^-20 rad; the tolerance adds twice that."""
+    pos = torch.tensor([2 ** 33 - 1, 2 ** 32 + 12345, -(2 ** 31) - 7, -1, 0], device="cuda")
+    freq = torch.from_numpy(tb.rope_freqs(64)[0]).cuda()
+    x = _randn(_gen(6), 5, 2, 64)
+    out = torch.empty_like(x)
+    assert lib.tcb_op_rope(_p(x), 128, 64, tb.F32, _p(pos), 1, tb.I64, _p(freq), 1.0, 64, 0, 0, _p(out), 128, 64, 5, 2, 64,
+                           _stream()) == 0
+    want, mag = rope_ref(x.double(), pos, freq, 1.0, 64, False, False)
+    within(out, want, mag * (10 * U + 2.0 ** -19))
+
+
+def test_rope_turns_back_and_gradient(lib):
+    """inverse undoes the turn, and is the gradient: <turn(x), w> and <x, inverse(w)> are equal, also against differences."""
+    g = _gen(8)
+    M, H, hd, rot = 9, 3, 48, 32
+    x, w, d = _randn(g, M, H * hd), _randn(g, M, H * hd), _randn(g, M, H * hd)
+    pos = torch.arange(M, device="cuda", dtype=torch.int32) * 100
+    freq = torch.from_numpy(tb.rope_freqs(rot)[0]).cuda()
+
+    def turn(v, inverse):
+        o = torch.empty_like(v)
+        assert lib.tcb_op_rope(_p(v), H * hd, hd, tb.F32, _p(pos), 1, tb.I32, _p(freq), 1.5, rot, 1, inverse, _p(o), H * hd, hd,
+                               M, H, hd, _stream()) == 0
+        return o
+
+    back = turn(turn(x, 0), 1).view(M, H, hd)
+    want = x.view(M, H, hd).double().clone()
+    want[..., :rot] *= 1.5 ** 2
+    within(back, want, 2.25 * 40 * U * 2 * x.abs().max().item())
+    grad = turn(w, 1).double()
+    n = M * H * hd
+    scale = (w.double().norm() * d.double().norm()).item() * 1.5
+    lhs = (turn(d, 0).double() * w.double()).sum()  # the turn is linear: its difference along d
+    assert abs((lhs - (grad * d.double()).sum()).item()) <= scale * 20 * U
+    eps = 2.0 ** -8
+    diff = (turn(x + eps * d, 0).double() - turn(x - eps * d, 0).double()) / (2 * eps)
+    assert abs((diff * w.double()).sum().item() - (grad * d.double()).sum().item()) <= n ** 0.5 * scale * 20 * U / eps
+
+
+def test_rope_far_pitch(lib):
+    ld = 1_300_000_008
+    buf = torch.empty(2 * ld + 64, dtype=torch.bfloat16, device="cuda")
+    x = buf.as_strided((3, 2, 32), (ld, 32, 1))
+    x.copy_(_randn(_gen(9), 3, 2, 32))
+    pos = torch.tensor([1, 2, 3], device="cuda", dtype=torch.int32)
+    freq = torch.from_numpy(tb.rope_freqs(32)[0]).cuda()
+    want, mag = rope_ref(x.double(), pos, freq, 1.0, 32, False, False)
+    assert lib.tcb_op_rope(_p(buf), ld, 32, tb.BF16, _p(pos), 1, tb.I32, _p(freq), 1.0, 32, 0, 0, _p(buf), ld, 32, 3, 2, 32,
+                           _stream()) == 0
+    within(x, want.to(torch.bfloat16), mag * 10 * U + want.abs() * 2.0 ** -7)
+
+
+# ------------------------------------------------------------------ 4-bit product
+def w4_case(lib, M, N, K, group, xtype, otype, xgroup=0, relu=False, res=False, bias=True, pad=0, seed=0, in_place=False):
+    g = _gen(seed + M + 3 * N + 5 * K)
+    ng = -(-K // group)
+    codes = torch.randint(-8, 8, (N, K), device="cuda", generator=g, dtype=torch.int8)
+    scales = ((0.5 + torch.rand(N, ng, device="cuda", generator=g)) / K ** 0.5).to(torch.bfloat16)
+    w = torch.from_numpy(tb.w4_pack(codes.cpu().numpy(), group, scales.float().cpu().numpy())).cuda()
+    wd = codes.double() * scales.double().repeat_interleave(group, 1)[:, :K]
+    x = _randn(g, M, K + pad)
+    xs = None
+    if xtype in TOP:
+        x = (x * TOP[xtype] / 4).clamp(-TOP[xtype], TOP[xtype])
+        xs = 0.01 + torch.rand(M, -(-K // xgroup) if xgroup else 1, device="cuda", generator=g) / TOP[xtype]
+    x = (x.round() if xtype == tb.I8 else x).to(TYPE[xtype])
+    xd = x[:, :K].double()
+    if xs is not None:
+        xd = xd * (xs.double().repeat_interleave(xgroup, 1)[:, :K] if xgroup else xs.double())
+    b = 0.1 * _randn(g, N) if bias else None
+    y = torch.full((M + 1, N + pad), 77.0, device="cuda").to(TYPE[otype])
+    r = _randn(g, M, N + pad).to(TYPE[otype]) if res else None
+    if in_place:
+        y[:M] = r
+        r = y
+    want, mag = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    if bias:
+        want, mag = want + b.double(), mag + b.double().abs()
+    if relu:
+        want = want.relu()
+    if res:
+        rd = r[:M, :N].double()
+        want, mag = want + rd, mag + rd.abs()
+    edge = y[:, N:].clone()
+    assert lib.tcb_op_gemv_w4(_p(x), K + pad, xtype, _p(xs), xgroup, _p(w), group, _p(b), int(relu), _p(r), N + pad, _p(y),
+                              N + pad, otype, M, N, K, _stream()) == 0
+    torch.cuda.synchronize()
+    tol = mag * (K + K / 16 + 16) * 2 * U + want.abs() * 2 * HALF[otype] + TINY[otype]
+    within(y[:M, :N], want.to(TYPE[otype]), tol)
+    assert torch.equal(y[:, N:], edge) and (y[M] == 77).all()
+    # the bound grows with K; the typical error does not: 99% within a few roundings of the magnitudes' root
+    err = (y[:M, :N].double() - want).abs()
+    usual = (want.abs() * 2 * HALF[otype] + mag * 16 * U + TINY[otype])
+    assert (err <= usual).double().mean().item() >= 0.99
+
+
+W4_SIZES = [(1, 1, 1), (1, 16, 128), (1, 128, 2560), (2, 17, 129), (3, 100, 31), (8, 640, 640), (9, 48, 1000), (16, 33, 512),
+            (17, 1920, 640), (1, 2560, 1280), (31, 65, 4096), (40, 130, 640), (64, 31, 300), (65, 64, 640), (130, 48, 256),
+            (1, 7, 16385), (5, 16, 20000), (1, 5000, 128), (33, 4099, 250)]
+
+
+@pytest.mark.parametrize("M,N,K", W4_SIZES)
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_gemv_w4(lib, M, N, K, group):
+    w4_case(lib, M, N, K, group, tb.BF16, tb.BF16)
+    w4_case(lib, M, N, K, group, tb.F16, tb.F32, relu=True, pad=1)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 48, 640), (4, 33, 1000), (13, 100, 250), (40, 1920, 640), (67, 17, 130)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("xgroup", [0, 32, 64, 128])
+@pytest.mark.parametrize("xtype", [tb.I8, tb.E4M3])
+def test_gemv_w4_codes(lib, M, N, K, group, xgroup, xtype):
+    w4_case(lib, M, N, K, group, xtype, tb.F32, xgroup=xgroup)
+    w4_case(lib, M, N, K, group, xtype, tb.BF16, xgroup=xgroup, res=True, pad=3)
+
+
+def test_gemv_w4_epilogues(lib):
+    for otype in (tb.BF16, tb.F16, tb.F32):
+        w4_case(lib, 5, 100, 640, 64, tb.BF16, otype, relu=True, res=True, bias=False)
+        w4_case(lib, 5, 100, 640, 64, tb.F16, otype, res=True, in_place=True, pad=4)
+        w4_case(lib, 20, 257, 384, 128, tb.F16, otype, bias=False)
+
+
+def test_gemv_w4_largest(lib):
+    w4_case(lib, 3, 16384, 8192, 128, tb.BF16, tb.BF16)
+    w4_case(lib, 32, 4096, 16384, 64, tb.F16, tb.F16)
+
+
+def test_gemv_w4_nan_and_inf_stay_in_their_row(lib):
+    """A NaN or an infinity in one token reaches that token's outputs only (a code of zero times infinity is NaN)."""
+    g = _gen(2)
+    x = _randn(g, 5, 256).to(torch.bfloat16)
+    x[1, 3], x[3, 255] = float("nan"), float("inf")
+    codes = torch.randint(1, 8, (32, 256), generator=torch.Generator().manual_seed(1), dtype=torch.int8)
+    w = torch.from_numpy(tb.w4_pack(codes.numpy(), 64, np.ones((32, 4), np.float32))).cuda()
+    y = torch.zeros(5, 32, device="cuda")
+    assert lib.tcb_op_gemv_w4(_p(x), 256, tb.BF16, None, 0, _p(w), 64, None, 0, None, 0, _p(y), 32, tb.F32, 5, 32, 256,
+                              _stream()) == 0
+    assert torch.isnan(y[1]).all() and torch.isposinf(y[3]).all() and torch.isfinite(y[[0, 2, 4]]).all()
+
+
+# ------------------------------------------------------------------ together
+def test_zero_rows_are_a_no_op(lib):
+    x = torch.ones(64, device="cuda", dtype=torch.bfloat16)
+    assert lib.tcb_op_rmsnorm(None, 64, None, 0, None, 0, None, 1e-6, tb.BF16, None, 64, tb.BF16, None, 0, 0, 64, _stream()) == 0
+    assert lib.tcb_op_rope(None, 64, 32, tb.BF16, None, 1, tb.F32, None, 1.0, 32, 0, 0, None, 64, 32, 0, 2, 32, _stream()) == 0
+    assert lib.tcb_op_gemv_w4(None, 64, tb.BF16, None, 0, None, 64, None, 0, None, 0, None, 8, tb.BF16, 0, 8, 64, _stream()) == 0
+    torch.cuda.synchronize()
+    assert (x == 1).all()
+
+
+class Block:
+    """The front of a pre-norm block on one packed stream: h = x + res, n = norm(h) in 8 bits, qkv = W4 n, q and k turned in
+    place by the records' day of year, attention over series of T tokens."""
+
+    def __init__(self, P, T, seed, code=tb.E4M3):
+        g = _gen(seed)
+        self.P, self.T, self.M, self.code = P, T, P * T, code
+        M = self.M
+        self.x, self.res = _randn(g, M, 640).to(torch.bfloat16), _randn(g, M, 640).to(torch.bfloat16)
+        self.g = 1 + 0.1 * _randn(g, 640)
+        self.rec = torch.randint(1, 367, (M, 11), device="cuda", generator=g).float()
+        self.freq = torch.from_numpy(tb.rope_freqs(160)[0]).cuda()
+        self.wf = (_randn(g, 1920, 640) / 640 ** 0.5).cpu().numpy()
+        self.w = torch.from_numpy(tb.w4_pack(self.wf, 64)).cuda()
+        self.bias = 0.1 * _randn(g, 1920)
+        self.h = torch.zeros_like(self.x)
+        self.n = torch.zeros(M, 640, device="cuda", dtype=TYPE[code])
+        self.s = torch.zeros(M, 5, device="cuda")
+        self.qkv = torch.zeros(M, 1920, device="cuda", dtype=torch.bfloat16)
+        self.before = torch.zeros_like(self.qkv)
+        self.att = torch.zeros_like(self.x)
+
+    def run(self, lib, stream=None):
+        st = stream or _stream()
+        M = self.M
+        assert lib.tcb_op_rmsnorm(_p(self.x), 640, _p(self.res), 640, _p(self.h), 640, _p(self.g), 1e-6, tb.BF16, _p(self.n),
+                                  640, self.code, _p(self.s), 128, M, 640, st) == 0
+        for out in (self.qkv, self.before):
+            assert lib.tcb_op_gemv_w4(_p(self.n), 640, self.code, _p(self.s), 128, _p(self.w), 64, _p(self.bias), 0, None, 0,
+                                      _p(out), 1920, tb.BF16, M, 1920, 640, st) == 0
+        assert lib.tcb_op_rope(_p(self.qkv), 1920, 160, tb.BF16, self.rec.data_ptr() + 40, 11, tb.F32, _p(self.freq), 1.0, 160, 0,
+                               0, _p(self.qkv), 1920, 160, M, 8, 160, st) == 0
+        assert lib.tcb_op_attention(_p(self.qkv), None, self.T, self.P, self.T, _p(self.att), st) == 0
+
+    def check(self):
+        from test_gpu_ops import attention_ref, close_bf16
+        from test_token_ops import unpack
+        h, v = rms_ref(self.x, self.res, self.g, 1e-6)
+        assert torch.equal(self.h, h)
+        check_rms(h, v, self.n, self.code, 128, self.s)
+        q, s = unpack(self.w.cpu().numpy(), 1920, 640, 64)
+        wd = torch.from_numpy(q * np.repeat(s, 64, 1).astype(np.float64)).cuda()
+        xd = self.n.double() * self.s.double().repeat_interleave(128, 1)
+        want, mag = xd @ wd.t() + self.bias.double(), xd.abs() @ wd.abs().t() + self.bias.double().abs()
+        within(self.before, want.to(torch.bfloat16), mag * 700 * 2 * U + want.abs() * 2.0 ** -7)
+        # against the weights before quantisation: 4 bits move a product's sum by its own rounding, at most half a scale
+        # (max|w| / 14 of a group) per term
+        assert ((want - xd @ torch.from_numpy(self.wf).cuda().double().t() - self.bias.double()).abs()
+                <= xd.abs() @ torch.from_numpy(np.repeat(s, 64, 1) * 0.54).cuda().double().t()).all()
+        M = self.M
+        turned, mag = rope_ref(self.before[:, :1280].double().view(M, 8, 160), self.rec[:, 10], self.freq, 1.0, 160, False, False)
+        within(self.qkv[:, :1280].view(M, 8, 160), turned.to(torch.bfloat16), mag * 10 * U + turned.abs() * 2.0 ** -7)
+        assert torch.equal(self.qkv[:, 1280:], self.before[:, 1280:])
+        close_bf16(self.att, attention_ref(self.qkv, np.arange(self.P + 1) * self.T), ulps=3, atol=1e-2)
+
+
+@pytest.mark.parametrize("P,T,code", [(1, 1, tb.E4M3), (1, 40, tb.E4M3), (3, 8, tb.I8), (1, 120, tb.I8)])
+def test_block_front(lib, P, T, code):
+    b = Block(P, T, P + T, code)
+    b.run(lib)
+    torch.cuda.synchronize()
+    b.check()
+
+
+def test_block_front_captured_and_replayed(lib):
+    """Captured once, replayed on new inputs in the same buffers, while another block runs on a second stream."""
+    a, b = Block(2, 16, 1), Block(2, 16, 2)
+    a.run(lib)  # the attention kernels' first use sets their attributes
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        a.run(lib)
+    fresh = Block(2, 16, 3)
+    for name in ("x", "res", "rec"):
+        getattr(a, name).copy_(getattr(fresh, name))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        graph.replay()
+        with torch.cuda.stream(side):
+            b.run(lib)
+    torch.cuda.synchronize()
+    a.check()
+    b.check()
+
+
+def test_repeated_calls_give_the_same_bits(lib):
+    a = Block(1, 64, 5)
+    a.run(lib)
+    first = [t.clone() for t in (a.h, a.n.view(torch.int8), a.s, a.qkv, a.att)]
+    for _ in range(3):
+        a.run(lib)
+        for u, v in zip(first, (a.h, a.n.view(torch.int8), a.s, a.qkv, a.att)):
+            assert torch.equal(u, v)
