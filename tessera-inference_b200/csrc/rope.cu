@@ -1,4 +1,8 @@
 // Rotary positions on the heads of token rows.
+//
+// Bound: HBM; every element is read and written once. A thread owns one unit of
+// a row, the same columns in every head, so that the cosines and sines of its
+// pairs are computed once per row and used by all heads.
 #include <algorithm>
 
 #include "token_ops.cuh"
@@ -6,55 +10,130 @@
 namespace tcb {
 namespace {
 
+constexpr int ROPE_THREADS = 256;
+constexpr int ROPE_AHEAD = 4;  // heads whose loads a thread issues together
+
 // cos and sin (times mscale) of pos * freq. The angle is reduced to a fraction
 // of a turn in f64, so a far position keeps its phase; the fraction is then
 // within half a turn, where f32 holds it to 2^-26 turns.
-template <class P>
-__device__ __forceinline__ float2 turn_of(P pos, double freq, float mscale, float sign) {
-    const double turns = (double)pos * freq * 0.15915494309189533577;  // 1 / (2 pi)
+__device__ __forceinline__ float2 turn_of(double pos, double freq, float mscale, float sign) {
+    const double turns = pos * freq * 0.15915494309189533577;  // 1 / (2 pi)
     float s, c;
     sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
     return make_float2(c * mscale, s * mscale * sign);
 }
 
-// One thread per (row, pair or copied column), over the heads.
-template <class T, class P, bool INTER>
-__global__ void __launch_bounds__(256) k_rope(RopeArgs a) {
-    const int half = a.rot / 2, units = half + a.hd - a.rot;
-    const int64_t n = a.M * units;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / units;
-        const int u = (int)(i - r * units);
+// V elements at once: 16 bytes, or a single element.
+template <class T, int V>
+struct Vec {
+    T v[V];
+};
+template <class T, int V>
+__device__ __forceinline__ Vec<T, V> load(const T *p) {
+    Vec<T, V> r;
+    if constexpr (V == 1) r.v[0] = *p;
+    else {
+        const uint4 q = *reinterpret_cast<const uint4 *>(p);
+        memcpy(&r, &q, 16);
+    }
+    return r;
+}
+template <class T, int V>
+__device__ __forceinline__ void store(T *p, const Vec<T, V> &r) {
+    if constexpr (V == 1) *p = r.v[0];
+    else {
+        uint4 q;
+        memcpy(&q, &r, 16);
+        *reinterpret_cast<uint4 *>(p) = q;
+    }
+}
+
+// Units of a row: first those that turn, then those that are copied (none when
+// out is x). A turning unit is two vectors of V first and V second elements of
+// the pairs (rot/2 apart), or, interleaved, two neighbouring vectors of V/2 pairs
+// each (one element each for V = 1): V pairs either way. blockIdx.y is a slice
+// of the heads.
+template <class T, class P, bool INTER, int V>
+__global__ void __launch_bounds__(ROPE_THREADS) k_rope(RopeArgs a, int units, int rows, int slice) {
+    const int half = a.rot / 2, turning = half / V;
+    const int h0 = blockIdx.y * slice, h1 = min(a.heads, h0 + slice);
+    const int rl = units < ROPE_THREADS ? threadIdx.x / units : 0;
+    if (rl >= rows) return;
+    for (int64_t r = (int64_t)blockIdx.x * rows + rl; r < a.M; r += (int64_t)gridDim.x * rows) {
         const T *x = static_cast<const T *>(a.x) + r * a.ldx;
         T *o = static_cast<T *>(a.out) + r * a.ldo;
-        if (u < half) {
-            const float2 t = turn_of(static_cast<const P *>(a.pos)[r * a.pos_stride], a.freq[u], a.mscale, a.sign);
-            const int p = INTER ? 2 * u : u, q = INTER ? p + 1 : u + half;
-            for (int h = 0; h < a.heads; ++h) {
-                const float v = to_f32(x[h * a.hsx + p]), w = to_f32(x[h * a.hsx + q]);
-                o[h * a.hso + p] = from_f32<T>(v * t.x - w * t.y);
-                o[h * a.hso + q] = from_f32<T>(v * t.y + w * t.x);
+        for (int u = threadIdx.x - rl * units; u < units; u += ROPE_THREADS) {
+            if (u >= turning) {
+                const int c = a.rot + (u - turning) * V;
+                for (int h = h0; h < h1; ++h) store<T, V>(o + h * a.hso + c, load<T, V>(x + h * a.hsx + c));
+                continue;
             }
-        } else {
-            const int c = u - half + a.rot;
-            for (int h = 0; h < a.heads; ++h) o[h * a.hso + c] = x[h * a.hsx + c];
+            const int p = INTER ? 2 * V * u : V * u, q = INTER ? p + V : p + half;
+            float2 t[V];
+            const double pos = (double)static_cast<const P *>(a.pos)[r * a.pos_stride];
+#pragma unroll
+            for (int j = 0; j < V; ++j) t[j] = turn_of(pos, a.freq[u * V + j], a.mscale, a.sign);
+            for (int h = h0; h < h1; h += ROPE_AHEAD) {
+                Vec<T, V> b[ROPE_AHEAD], c[ROPE_AHEAD];
+#pragma unroll
+                for (int k = 0; k < ROPE_AHEAD; ++k)
+                    if (h + k < h1) {
+                        b[k] = load<T, V>(x + (h + k) * a.hsx + p);
+                        c[k] = load<T, V>(x + (h + k) * a.hsx + q);
+                    }
+#pragma unroll
+                for (int k = 0; k < ROPE_AHEAD; ++k) {
+                    if (h + k >= h1) break;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        // pair j: element j of both vectors, or elements 2j and 2j + 1 of the two in a row
+                        T &v = INTER && V > 1 ? (2 * j < V ? b[k].v[2 * j % V] : c[k].v[2 * j % V]) : b[k].v[j];
+                        T &w = INTER && V > 1 ? (2 * j < V ? b[k].v[(2 * j + 1) % V] : c[k].v[(2 * j + 1) % V]) : c[k].v[j];
+                        const float f = to_f32(v), g = to_f32(w);
+                        v = from_f32<T>(f * t[j].x - g * t[j].y);
+                        w = from_f32<T>(f * t[j].y + g * t[j].x);
+                    }
+                    store<T, V>(o + (h + k) * a.hso + p, b[k]);
+                    store<T, V>(o + (h + k) * a.hso + q, c[k]);
+                }
+            }
         }
     }
 }
 
+template <class T, class P, bool INTER, int V>
+void launch(const RopeArgs &a, cudaStream_t st) {
+    const int units = a.rot / 2 / V + (a.out == a.x ? 0 : (a.hd - a.rot) / V);
+    const int rows = std::max(1, ROPE_THREADS / units);
+    const int64_t blocks = (a.M + rows - 1) / rows;
+    // With few rows the heads are spread over the grid too, at the price of the angles' being computed again.
+    const int64_t spread = std::min<int64_t>(a.heads, std::max<int64_t>(1, 148 / blocks));
+    const int slice = (int)((a.heads + spread - 1) / spread);
+    const dim3 grid((unsigned)std::min<int64_t>(blocks, 1 << 30), (a.heads + slice - 1) / slice);
+    k_rope<T, P, INTER, V><<<grid, ROPE_THREADS, 0, st>>>(a, units, rows, slice);
+}
+
 template <class T, class P>
-void launch(const RopeArgs &a, bool inter, cudaStream_t st) {
-    const int64_t n = a.M * (a.hd - a.rot / 2);
-    const unsigned grid = (unsigned)std::min<int64_t>((n + 255) / 256, 1 << 20);
-    if (inter) k_rope<T, P, true><<<grid, 256, 0, st>>>(a);
-    else k_rope<T, P, false><<<grid, 256, 0, st>>>(a);
+void launch_v(const RopeArgs &a, bool inter, cudaStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    const auto at = [](const void *p, int64_t ld, int64_t hs) {
+        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % V == 0 && hs % V == 0;
+    };
+    // the pairs, the copied columns, and every row and head in whole vectors
+    if (a.rot / 2 % V == 0 && (a.hd - a.rot) % V == 0 && at(a.x, a.ldx, a.hsx) && at(a.out, a.ldo, a.hso)) {
+        if (inter) launch<T, P, true, V>(a, st);
+        else launch<T, P, false, V>(a, st);
+    } else {
+        if (inter) launch<T, P, true, 1>(a, st);
+        else launch<T, P, false, 1>(a, st);
+    }
 }
 
 template <class T>
 void launch_p(const RopeArgs &a, int pos_type, bool inter, cudaStream_t st) {
-    if (pos_type == TCB_F32) launch<T, float>(a, inter, st);
-    else if (pos_type == TCB_I32) launch<T, int32_t>(a, inter, st);
-    else launch<T, int64_t>(a, inter, st);
+    if (pos_type == TCB_F32) launch_v<T, float>(a, inter, st);
+    else if (pos_type == TCB_I32) launch_v<T, int32_t>(a, inter, st);
+    else launch_v<T, int64_t>(a, inter, st);
 }
 
 }  // namespace
