@@ -65,8 +65,8 @@ def test_rope_refusals(kw, says, capfd):
 
 
 @pytest.mark.parametrize("kw,says", [
-    (dict(xtype=tb.F32), "xtype"), (dict(xtype=tb.I32), "xtype"), (dict(otype=tb.E4M3), "otype"), (dict(M=-1), "M is negative"),
-    (dict(N=0), "N < 1"), (dict(K=0), "K is not"), (dict(K=2 ** 20 + 1, ldx=2 ** 20 + 1), "K is not"),
+    (dict(xtype=tb.F32), "xtype"), (dict(xtype=tb.I32), "xtype"), (dict(otype=tb.E4M3), "otype"), (dict(M=-1), "M is not"), (dict(M=2 ** 18 + 1), "M is not"),
+    (dict(N=0), "N < 1"), (dict(K=0), "K is not"), (dict(K=65537, ldx=65537), "K is not"),
     (dict(group=16), "group"), (dict(group=0), "group"), (dict(xgroup=16), "xgroup"),
     (dict(xtype=tb.BF16, xscales=None, xgroup=32), "xgroup without"), (dict(xtype=tb.BF16), "xscales without"),
     (dict(xscales=None), "xscales is NULL"), (dict(ldx=255), "pitch"), (dict(ldo=47), "pitch"), (dict(ldr=47), "pitch"),
@@ -168,7 +168,7 @@ def test_w4_pack_quantises(N, K, group):
 
 def test_w4_pack_refusals(capfd):
     lib = tb.load_library()
-    for bad in ((0, 128, 32), (16, 0, 32), (16, 128, 16), (16, 2 ** 20 + 1, 32), (-1, 128, 32)):
+    for bad in ((0, 128, 32), (16, 0, 32), (16, 128, 16), (16, 65537, 32), (-1, 128, 32)):
         assert lib.tcb_w4_bytes(*bad) == -1
         assert lib.tcb_w4_pack(P, *bad, P) == -1
         assert lib.tcb_w4_pack_codes(P, P, *bad, P) == -1
