@@ -1,0 +1,8 @@
+// Root-mean-square norm: the kernels for f16 rows.
+#include "rmsnorm.cuh"
+
+namespace tcb {
+
+void rms_launch_f16(const RmsArgs &a, int ytype, bool vec, cudaStream_t st) { rms_launch_type<f16>(a, ytype, vec, st); }
+
+}  // namespace tcb
