@@ -1,19 +1,30 @@
 // Linear of a few token rows with 4-bit weights and group scales.
 //
-// Bound: the bytes of the weights, read once per tile of up to 32 token rows.
-// The products run on mma.sync m16n8k16: 16 weight rows are its M side, 8 token
-// rows its N side. With one to 32 columns on that side the tensor pipe has
-// nothing to win, the weights' codes arrive in the order of the instruction's
-// A operand, and a pair of codes becomes two 16-bit floats with a shift, a logic
-// and a subtract instruction. A code times an activation is exact in f32, where
-// the sums are kept; a group's sum is multiplied by its scale in f32.
+// Bound: the bytes of the weights for up to 8 token rows, mma.sync above. The
+// products run on mma.sync m16n8k16: 16 weight rows are its M side, 8 token rows
+// its N side, and the weights' codes arrive in the order of its A operand. What has
+// to be cheap is turning codes into 16-bit floats:
+//
+//   u = q + 8 in the low bits of an fp16 is the subnormal u 2^-24, in bits 4-7 it is
+//   16 u 2^-24, both exact. So a logic instruction per pair, and a shift per eight
+//   codes, are all; the two kinds of pairs go to sums of their own, X and Y, and a
+//   group's sum is 2^24 (X + Y / 16) - 8 (sum of the group's x). The last term is
+//   the same for all weight rows: it is summed once per block and X starts with it.
+//
+// The token rows are staged as fp16. That is exact for fp16, int8 and e4m3. A group
+// of a bf16 row is scaled by a power of two that takes its largest finite value to
+// 2^14 or above, which is exact down to 2^-31 of that value and rounds what is
+// smaller by at most 2^-39 of it, far below what f32 sums of these terms round.
+// Products are exact and sums are f32; a group's sum is multiplied by its scale in
+// f32. An infinity or a NaN among the activations ends as NaN in X: where the result
+// is NaN, it is computed again from the definition, one product after the other.
 //
 // One block of 16 warps per SM stays for the whole call. It keeps its token rows
 // in shared memory and streams weight records, each warp through a ring of its
-// own, filled by asynchronous copies that run on across the ends of tiles. Where
-// the token rows of all K columns are large beside a block's share of the
-// weights, a cluster of 2, 4 or 8 blocks splits K, and each block stages only its
-// slice; the sums of the slices are joined over distributed shared memory.
+// own, filled by asynchronous copies that start before the token rows are there and
+// run on across the ends of tiles. A cluster of 2, 4 or 8 blocks may split K, where
+// the token rows of all K columns are too many for a block or the weight rows too
+// few for the SMs; the sums of the slices are joined over distributed shared memory.
 #include <algorithm>
 #include <atomic>
 
@@ -25,63 +36,17 @@ namespace tcb {
 namespace {
 
 constexpr int W4_WARPS = 16, W4_THREADS = W4_WARPS * 32;
-constexpr int W4_RING = 4;   // records in flight per warp
-constexpr int X_PAD = 32;    // 16-bit elements behind a staged token row: rows start 16 banks apart
-constexpr int X_SMALL = 32 * 1024, X_PART = 4;  // token rows of up to 32 KB, or a quarter of the weights' share, stay whole
+constexpr int X_PAD = 32;               // 16-bit elements behind a staged token row: rows start 16 banks apart
 constexpr int SMEM_MAX = 227 * 1024;
 
-template <class X>
-using mma_type = std::conditional_t<std::is_same_v<X, f16>, f16, bf16>;
-
-template <class T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (std::is_same_v<T, bf16>)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Codes q + 8 in nibbles p and p + 4 of w as two floats q. A code in the low bits of the significand of 128 (bf16) or
-// 1024 (fp16) adds exactly its value; 136 or 1032 is subtracted, exactly.
-template <class T>
-__device__ __forceinline__ uint32_t codes2(uint32_t w, int p) {
-    uint32_t v = w >> (4 * p);
-    if constexpr (std::is_same_v<T, bf16>) {
-        asm("lop3.b32 %0, %0, 0x000f000f, 0x43004300, 0xea;" : "+r"(v));  // (v & mask) | 128
-        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&v), __nv_bfloat162{bf16(136.f), bf16(136.f)});
-        return *reinterpret_cast<const uint32_t *>(&r);
-    } else {
-        asm("lop3.b32 %0, %0, 0x000f000f, 0x64006400, 0xea;" : "+r"(v));  // (v & mask) | 1024
-        const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&v), __half2{f16(1032.f), f16(1032.f)});
-        return *reinterpret_cast<const uint32_t *>(&r);
-    }
-}
-
-// 8 elements of x as the matrix instruction's type; 8-bit values are exact in bf16.
-template <class X>
-__device__ __forceinline__ uint4 as_mma8(const X *p) {
-    if constexpr (sizeof(X) == 2) return *reinterpret_cast<const uint4 *>(p);
-    const uint2 q = *reinterpret_cast<const uint2 *>(p);
-    X v[8];
-    memcpy(v, &q, 8);
-    return make_uint4(pack_bf16x2(to_f32(v[0]), to_f32(v[1])), pack_bf16x2(to_f32(v[2]), to_f32(v[3])),
-                      pack_bf16x2(to_f32(v[4]), to_f32(v[5])), pack_bf16x2(to_f32(v[6]), to_f32(v[7])));
-}
-template <class X>
-__device__ __forceinline__ mma_type<X> as_mma1(X v) {
-    if constexpr (sizeof(X) == 2) return v;
-    else return __float2bfloat16_rn(to_f32(v));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -93,22 +58,74 @@ __device__ __forceinline__ uint4 lds128(uint32_t p) {
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
     return v;
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t p) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(p) : "memory");
+__device__ __forceinline__ float2 lds_f32x2(uint32_t p) {
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(p) : "memory");
     return v;
+}
+__device__ __forceinline__ float lds_bf16(uint32_t p) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(p) : "memory");
+    return bf16lo(v);
+}
+
+// 8 elements of x from element i on, as they are stored: 16-bit ones fill four words, 8-bit ones two. Elements from `end` on
+// are zero; `vec`: i is a multiple of 8 and rows start at 8-element boundaries.
+__device__ __forceinline__ uint4 x8(const void *x, int64_t i, int64_t end, bool wide, bool vec) {
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (vec && i + 8 <= end) {
+        if (wide) return *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(x) + i);
+        const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(x) + i);
+        return make_uint4(q.x, q.y, 0, 0);
+    }
+    if (wide) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i + j < end) w[j / 2] |= (uint32_t)static_cast<const uint16_t *>(x)[i + j] << 16 * (j % 2);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i + j < end) w[j / 4] |= (uint32_t)static_cast<const uint8_t *>(x)[i + j] << 8 * (j % 4);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // How a launch cuts the work. `split` blocks of a cluster share K; within a block the warps are 16 / wk row tiles times wk
-// slices of the records. Cluster c of `clusters` takes row tiles ((c + i clusters) (16 / wk)) + 0 .. in step i < steps.
+// slices of the records. Cluster c of `clusters` takes row tiles ((c + i clusters) (16 / wk)) + 0 .. in step i; after every
+// `steps` of them, `batches` times, a cluster joins its slices' sums.
 struct W4Cut {
-    int split = 1, wk = 1, clusters = 1, steps = 1;
-    int rows = 1;                                    // token rows of a full tile
-    int x_at = 0, xsc_at = 0, red_at = 0, part_at = 0;  // byte offsets in shared memory
-    bool vec = false;                                // x rows can be read in 8-element steps
+    int split = 1, wk = 1, clusters = 1, steps = 1, batches = 1;
+    int rows = 1;                                                    // token rows of a full tile
+    int x_at = 0, sums_at = 0, xsc_at = 0, red_at = 0, part_at = 0;  // byte offsets in shared memory
+    bool vec = false;                                                // x rows can be read in 8-element steps
 };
 
-__device__ __forceinline__ void put_out(const W4Args &a, int otype, int64_t m, int n, float v) {
+// Output (m, n) from the definition, for results that are NaN.
+__device__ __noinline__ float w4_plain(const W4Args &a, int xtype, int64_t m, int n) {
+    const int kb = (a.K + W4_COLS - 1) / W4_COLS, rec = w4_record_bytes(a.group), r = n % W4_ROWS;
+    const int xg = a.xgroup ? a.xgroup : a.K, nxg = (a.K + xg - 1) / xg;
+    const uint8_t *w = static_cast<const uint8_t *>(a.w) + (int64_t)(n / W4_ROWS) * kb * rec;
+    float v = 0.f;
+#pragma unroll 1
+    for (int k = 0; k < a.K; ++k) {
+        const int j = k % W4_COLS, i = j / 32, t = j / 8 % 4, c = j % 8, nib = c / 2 + 4 * (c % 2);
+        const uint8_t *p = w + (int64_t)(k / W4_COLS) * rec;
+        const int q = (p[512 * (r / 8) + 64 * (r % 8) + 16 * t + 4 * i + nib / 2] >> 4 * (nib % 2) & 15) - 8;
+        const float s = to_f32(reinterpret_cast<const bf16 *>(p + W4_CODE_BYTES)[j / a.group * W4_ROWS + r]);
+        const int64_t at = m * a.ldx + k;
+        float x;
+        if (xtype == TCB_BF16) x = to_f32(static_cast<const bf16 *>(a.x)[at]);
+        else if (xtype == TCB_F16) x = to_f32(static_cast<const f16 *>(a.x)[at]);
+        else if (xtype == TCB_I8) x = to_f32(static_cast<const int8_t *>(a.x)[at]);
+        else x = to_f32(static_cast<const e4m3 *>(a.x)[at]);
+        if (a.xscales) x *= a.xscales[m * nxg + k / xg];
+        v += x * (float)q * s;
+    }
+    return v;
+}
+
+__device__ __noinline__ void put_out(const W4Args &a, int xtype, int otype, int m, int n, float v) {
+    if (v != v) v = w4_plain(a, xtype, m, n);
     if (a.bias) v += a.bias[n];
     if (a.relu) v = v < 0.f ? 0.f : v;
     const int64_t at = m * a.ldo + n, ar = m * a.ldr + n;
@@ -124,10 +141,11 @@ __device__ __forceinline__ void put_out(const W4Args &a, int otype, int64_t m, i
     }
 }
 
-// X: type of x. SUB: columns whose products share both scales. NT: tiles of 8 token rows. XG: x's scales change along a row.
-template <class X, int SUB, int NT, bool XG>
-__global__ void __launch_bounds__(W4_THREADS, 1) k_gemv_w4(const W4Args a, const W4Cut cut, const int otype) {
-    using T = mma_type<X>;
+// SUB: columns whose products share both scales. NT: tiles of 8 token rows. XG: x has scales that change along a row, the
+// caller's or those of staged bf16. RING: records in flight per warp.
+template <int SUB, int NT, bool XG, int RING>
+__global__ void __launch_bounds__(W4_THREADS, 1)
+    k_gemv_w4(const __grid_constant__ W4Args a, const __grid_constant__ W4Cut cut, const int xtype, const int otype) {
     extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int wt = W4_WARPS / cut.wk, my_t = warp / cut.wk, my_k = warp % cut.wk;
@@ -135,183 +153,221 @@ __global__ void __launch_bounds__(W4_THREADS, 1) k_gemv_w4(const W4Args a, const
     const int cluster = blockIdx.x / cut.split, rank = blockIdx.x % cut.split;
     const int b0 = (int)((int64_t)kb * rank / cut.split), b1 = (int)((int64_t)kb * (rank + 1) / cut.split);
     const int m0 = blockIdx.y * cut.rows, rows = min(cut.rows, a.M - m0);
-    const int count = (b1 - b0 - my_k + cut.wk - 1) / cut.wk;  // records of this warp in a tile, at least 1
+    // records of this warp in a tile, at least one, in a row
+    const int r0 = (b1 - b0) * my_k / cut.wk, count = (b1 - b0) * (my_k + 1) / cut.wk - r0;
 
-    // the ring: a warp's lanes copy what they read themselves, so no lane waits for another
-    const uint32_t ring = smem_u32(smem) + warp * W4_RING * rec;
-    const int words = W4_COLS / a.group * W4_ROWS / 2;  // scales of a record, two to a word: one word per lane
-    int f_step = 0, f_rec = 0, f_slot = 0;
+    // This slice of the token rows: 32 times 8 columns of a row per warp and pass, zero behind the last column. The first
+    // pass's loads go out before the weights', and every pass's before the one in front is worked on.
+    const int pitch = (kb + cut.split - 1) / cut.split * W4_COLS + X_PAD, k0 = b0 * W4_COLS, kn = (b1 - b0) * W4_COLS;
+    const int passes = (kn + 255) / 256;
+    const bool wide = xtype == TCB_BF16 || xtype == TCB_F16;
+    const auto x_load = [&](int e) {
+        const int m = e / passes, k = (e - m * passes) * 256 + lane * 8;
+        const int64_t row = (int64_t)(m0 + m) * a.ldx;
+        if (e >= rows * passes || k >= kn) return make_uint4(0, 0, 0, 0);
+        return x8(a.x, row + k0 + k, row + a.K, wide, cut.vec);
+    };
+    uint4 ahead = x_load(warp);
+
+    // the ring: a warp's lanes copy what they read themselves, but for the scales (lanes below `tail`, 16 bytes each)
+    const uint32_t ring = smem_u32(smem) + warp * RING * rec, ring_end = ring + RING * rec;
+    const int tail = (rec - W4_CODE_BYTES) / 16;
+    const int first = cluster * wt + my_t, hop = cut.clusters * wt;  // tiles of this warp: first, first + hop, ...
+    const uint8_t *f_src = static_cast<const uint8_t *>(a.w) + ((int64_t)first * kb + b0 + r0) * rec + lane * 16;
+    int f_left = first < tiles ? (tiles - first + hop - 1) / hop * count : 0, f_rec = count;
+    uint32_t f_dst = ring;
     const auto fetch = [&] {
-        const int tile = (cluster + f_step * cut.clusters) * wt + my_t;
-        if (f_step < cut.steps && tile < tiles) {
-            const uint8_t *p = static_cast<const uint8_t *>(a.w) + ((int64_t)tile * kb + b0 + my_k + f_rec * cut.wk) * rec;
-            const uint32_t d = ring + f_slot * rec;
-            cp_async16(d + lane * 16, p + lane * 16);
-            cp_async16(d + 512 + lane * 16, p + 512 + lane * 16);
-            if (lane < words) cp_async4(d + W4_CODE_BYTES + lane * 4, p + W4_CODE_BYTES + lane * 4);
+        if (f_left > 0) {
+            cp_async16(f_dst + lane * 16, f_src);
+            cp_async16(f_dst + 512 + lane * 16, f_src + 512);
+            if (lane < tail) cp_async16(f_dst + W4_CODE_BYTES + lane * 16, f_src + W4_CODE_BYTES);
+            --f_left;
+            f_src += rec;
+            if (--f_rec == 0) f_rec = count, f_src += ((int64_t)hop * kb - count) * rec;
+            f_dst = f_dst + rec == ring_end ? ring : f_dst + rec;
         }
         cp_async_commit();
-        if (++f_rec == count) f_rec = 0, ++f_step;
-        f_slot = f_slot + 1 == W4_RING ? 0 : f_slot + 1;
     };
-#pragma unroll
-    for (int s = 0; s < W4_RING - 1; ++s) fetch();
+#pragma unroll 1
+    for (int s = 0; s < RING - 1; ++s) fetch();
 
-    // this slice of the token rows, zero behind the last column
-    const int pitch = (kb + cut.split - 1) / cut.split * W4_COLS + X_PAD, k0 = b0 * W4_COLS, kn = (b1 - b0) * W4_COLS;
-    T *xs = reinterpret_cast<T *>(smem + cut.x_at);
-    const X *x = static_cast<const X *>(a.x) + (int64_t)m0 * a.ldx;
-    if (cut.vec) {
-        const int per = kn / 8;
-        for (int e = threadIdx.x; e < rows * per; e += W4_THREADS) {
-            const int m = e / per, k = (e - m * per) * 8;
-            const X *p = x + m * a.ldx + k0 + k;
-            uint4 v;
-            if (k0 + k + 8 <= a.K) v = as_mma8(p);
-            else {
-                T u[8];
-                for (int j = 0; j < 8; ++j) u[j] = k0 + k + j < a.K ? as_mma1(p[j]) : T(0.f);
-                memcpy(&v, u, 16);
+    uint16_t *xs = reinterpret_cast<uint16_t *>(smem + cut.x_at);
+    float *sums = reinterpret_cast<float *>(smem + cut.sums_at), *xsc = reinterpret_cast<float *>(smem + cut.xsc_at);
+#pragma unroll 1
+    for (int e = warp; e < rows * passes; e += W4_WARPS) {
+        const uint4 v = ahead;
+        ahead = x_load(e + W4_WARPS);
+        const int m = e / passes, k = (e - m * passes) * 256 + lane * 8;
+        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        float f[8], back = 1.f;
+        if (xtype == TCB_BF16) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t lo = w[j] << 16 & 0x7fff0000u, hi = w[j] & 0x7fff0000u;
+                top = max(top, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
             }
-            *reinterpret_cast<uint4 *>(xs + m * pitch + k) = v;
+#pragma unroll
+            for (int o = 1; o < SUB / 8; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+            // 2^(14 - exponent of the largest value), in two factors that f32 holds; back is its inverse times 2^24
+            const int up = 14 - max((int)(top >> 23) - 127, -126);
+            const float f0 = __uint_as_float((uint32_t)(up / 2 + 127) << 23), f1 = __uint_as_float((uint32_t)(up - up / 2 + 127) << 23);
+            back = __uint_as_float((uint32_t)(127 - up / 2) << 23) * __uint_as_float((uint32_t)(127 - up + up / 2) << 23);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const __half2 h = __floats2half2_rn(bf16lo(w[j]) * f0 * f1, bf16hi(w[j]) * f0 * f1);
+                w[j] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+        } else if (!wide) {
+#pragma unroll
+            for (int j = 3; j >= 0; --j) {
+                const uint32_t b = w[j / 2] >> 16 * (j % 2) & 0xffffu;
+                __half2 h;
+                if (xtype == TCB_I8) h = __floats2half2_rn((float)(int8_t)b, (float)(int8_t)(b >> 8));
+                else h = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)b, __NV_E4M3));
+                w[j] = *reinterpret_cast<const uint32_t *>(&h);
+            }
         }
-    } else {
-        for (int m = 0; m < rows; ++m) {
-            const X *p = x + m * a.ldx + k0;
-#pragma unroll 4
-            for (int k = threadIdx.x; k < kn; k += W4_THREADS) xs[m * pitch + k] = k0 + k < a.K ? as_mma1(p[k]) : T(0.f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
+            f[2 * j] = h.x;
+            f[2 * j + 1] = h.y;
+        }
+        float sum = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+#pragma unroll
+        for (int o = 1; o < SUB / 8; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        if (k < kn) {
+            *reinterpret_cast<uint4 *>(xs + m * pitch + k) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (k % SUB == 0) {
+                const int at = k / SUB * 8 * NT + m;
+                sums[at] = sum * (-8.f * 0x1p-24f);
+                if constexpr (XG) {
+                    if (xtype != TCB_BF16) back = k0 + k < a.K ? __ldg(a.xscales + (int64_t)(m0 + m) * ((a.K + a.xgroup - 1) / a.xgroup) + (k0 + k) / a.xgroup) : 0.f;
+                    xsc[at] = back * 0x1p24f;
+                }
+            }
         }
     }
-    const int xg = a.xgroup ? a.xgroup : W4_COLS, xgs = kn / xg, nxg = (a.K + xg - 1) / xg;
-    float *xsc = reinterpret_cast<float *>(smem + cut.xsc_at);
-    if constexpr (XG)
-        for (int e = threadIdx.x; e < rows * xgs; e += W4_THREADS) {
-            const int m = e / xgs, k = k0 / xg + e - m * xgs;
-            xsc[e] = k < nxg ? a.xscales[(int64_t)(m0 + m) * nxg + k] : 0.f;
-        }
     __syncthreads();
 
     uint32_t brow[NT];  // lanes behind the last token row read it again; their sums are not written
 #pragma unroll
     for (int n = 0; n < NT; ++n) brow[n] = smem_u32(xs) + (min(8 * n + g, rows - 1) * pitch + 8 * t) * 2;
-
+    const uint32_t my_sums = smem_u32(sums) + 8 * t, my_xsc = smem_u32(xsc) + 8 * t;
     float *red = reinterpret_cast<float *>(smem + cut.red_at), *part = reinterpret_cast<float *>(smem + cut.part_at);
-    int slot = 0;
-    for (int step = 0; step < cut.steps; ++step) {
-        const int tile = (cluster + step * cut.clusters) * wt + my_t;
-        if (tile >= tiles) break;  // the same for all warps of a tile
-        float acc[NT][4] = {};
+    const int tile_floats = rows * W4_ROWS;
+    namespace cg = cooperative_groups;
+    const cg::cluster_group cl = cg::this_cluster();
+
+    uint32_t slot = ring;
+    int tile = first;
 #pragma unroll 1
-        for (int r = 0; r < count; ++r) {
-            cp_async_wait<W4_RING - 2>();
-            const uint32_t d = ring + slot * rec;
-            const uint4 lo = lds128(d + lane * 16), hi = lds128(d + 512 + lane * 16);
-            const uint32_t scales = lane < words ? lds32(d + W4_CODE_BYTES + lane * 4) : 0;
-            fetch();  // into the slot read in the round before
-            slot = slot + 1 == W4_RING ? 0 : slot + 1;
-            const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
-            const int kl = (my_k + r * cut.wk) * W4_COLS;
-            float sum[NT][4];
+    for (int batch = 0; batch < cut.batches; ++batch) {
+#pragma unroll 1
+        for (int step = 0; step < cut.steps && tile < tiles; ++step, tile += hop) {  // alike for all warps of a tile
+            float acc[NT][4] = {};
+#pragma unroll 1
+            for (int r = r0; r < r0 + count; ++r) {
+                cp_async_wait<RING - 2>();
+                __syncwarp();
+                const uint4 lo = lds128(slot + lane * 16), hi = lds128(slot + 512 + lane * 16);
+                float su[W4_COLS / SUB], sv[W4_COLS / SUB];  // scales of rows g and g + 8
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (j * 32 % SUB == 0) {
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) sum[n][c] = 0.f;
+                for (int j = 0; j < W4_COLS / SUB; ++j) {
+                    const uint32_t p = slot + W4_CODE_BYTES + (j * SUB / a.group * W4_ROWS + g) * 2;
+                    su[j] = lds_bf16(p);
+                    sv[j] = lds_bf16(p + 16);
                 }
-                uint32_t A[2][4];
+                fetch();  // into the slot read in the round before
+                slot = slot + rec == ring_end ? ring : slot + rec;
+                const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+                float X[NT][4], Y[NT][4];
 #pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    A[p / 2][p % 2 * 2] = codes2<T>(wl[j], p);
-                    A[p / 2][p % 2 * 2 + 1] = codes2<T>(wh[j], p);
-                }
+                for (int j = 0; j < 4; ++j) {
+                    const int sub = j * 32 / SUB;
+                    if (j * 32 % SUB == 0) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const uint4 b = lds128(brow[n] + (kl + 32 * j) * 2);
-                    mma16816<T>(sum[n], A[0], b.x, b.y);
-                    mma16816<T>(sum[n], A[1], b.z, b.w);
-                }
-                if ((j + 1) * 32 % SUB == 0) {
-                    const int word = j * 32 / a.group * (W4_ROWS / 2) + g / 2;
-                    const uint32_t u = __shfl_sync(~0u, scales, word), v = __shfl_sync(~0u, scales, word + 4);
-                    const float su = g % 2 ? bf16hi(u) : bf16lo(u), sv = g % 2 ? bf16hi(v) : bf16lo(v);
+                        for (int n = 0; n < NT; ++n) {
+                            const float2 s = lds_f32x2(my_sums + ((r * (W4_COLS / SUB) + sub) * 8 * NT + 8 * n) * 4);
+                            X[n][0] = X[n][2] = s.x;
+                            X[n][1] = X[n][3] = s.y;
+                            Y[n][0] = Y[n][1] = Y[n][2] = Y[n][3] = 0.f;
+                        }
+                    }
+                    const uint32_t vl = wl[j] >> 8, vh = wh[j] >> 8;
+                    const uint32_t A[4] = {wl[j] & 0x000f000fu, wh[j] & 0x000f000fu, vl & 0x000f000fu, vh & 0x000f000fu};
+                    const uint32_t B[4] = {wl[j] & 0x00f000f0u, wh[j] & 0x00f000f0u, vl & 0x00f000f0u, vh & 0x00f000f0u};
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        float x0 = 1.f, x1 = 1.f;
-                        if constexpr (XG) {
-                            const int k = (kl + 32 * j) / xg;
-                            x0 = xsc[min(8 * n + 2 * t, rows - 1) * xgs + k];
-                            x1 = xsc[min(8 * n + 2 * t + 1, rows - 1) * xgs + k];
+                        const uint4 b = lds128(brow[n] + (r * W4_COLS + 32 * j) * 2);
+                        mma16816(X[n], A, b.x, b.z);
+                        mma16816(Y[n], B, b.y, b.w);
+                    }
+                    if ((j + 1) * 32 % SUB == 0) {
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            float s0 = su[sub], s1 = su[sub], s2 = sv[sub], s3 = sv[sub];
+                            if constexpr (XG) {
+                                const float2 xf = lds_f32x2(my_xsc + ((r * (W4_COLS / SUB) + sub) * 8 * NT + 8 * n) * 4);
+                                s0 *= xf.x, s1 *= xf.y, s2 *= xf.x, s3 *= xf.y;
+                            }
+                            acc[n][0] = fmaf(fmaf(Y[n][0], 0.0625f, X[n][0]), s0, acc[n][0]);
+                            acc[n][1] = fmaf(fmaf(Y[n][1], 0.0625f, X[n][1]), s1, acc[n][1]);
+                            acc[n][2] = fmaf(fmaf(Y[n][2], 0.0625f, X[n][2]), s2, acc[n][2]);
+                            acc[n][3] = fmaf(fmaf(Y[n][3], 0.0625f, X[n][3]), s3, acc[n][3]);
                         }
-                        acc[n][0] = fmaf(sum[n][0], XG ? su * x0 : su, acc[n][0]);
-                        acc[n][1] = fmaf(sum[n][1], XG ? su * x1 : su, acc[n][1]);
-                        acc[n][2] = fmaf(sum[n][2], XG ? sv * x0 : sv, acc[n][2]);
-                        acc[n][3] = fmaf(sum[n][3], XG ? sv * x1 : sv, acc[n][3]);
                     }
                 }
             }
-        }
-        if constexpr (sizeof(X) == 1 && !XG) {
+            // Slices' sums meet in shared memory, in slice order. Two buffers in turn, so one barrier does; a warp that has
+            // its tile alone needs one buffer, or none when the cluster joins slices anyway.
+            float *joined = part + (step * wt + my_t) * tile_floats;
+            float *buf = cut.wk > 1 ? red + (((step & 1) * wt + my_t) * cut.wk + my_k) * tile_floats
+                         : cut.split > 1 ? joined : red + my_t * tile_floats;
+            __syncwarp();
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) acc[n][c] *= __ldg(a.xscales + m0 + min(8 * n + 2 * t + c % 2, rows - 1));
-        }
-        // value c of tile n is weight row g + 8 (c / 2), token row 8 n + 2 t + c % 2
-        if (cut.wk == 1) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int m = 8 * n + 2 * t + c % 2, i = g + c / 2 * 8;
-                    if (m >= rows) continue;
-                    if (cut.split > 1) part[((step * wt + my_t) * rows + m) * W4_ROWS + i] = acc[n][c];
-                    else if (tile * W4_ROWS + i < a.N) put_out(a, otype, m0 + m, tile * W4_ROWS + i, acc[n][c]);
+                for (int c = 0; c < 4; ++c) {  // weight row g + 8 (c / 2), token row 8 n + 2 t + c % 2
+                    const int m = 8 * n + 2 * t + c % 2;
+                    if (m < rows) buf[m * W4_ROWS + g + c / 2 * 8] = XG ? acc[n][c] : acc[n][c] * 0x1p24f;
                 }
-            continue;
-        }
-        // the slices' sums meet in shared memory, in slice order; two buffers in turn, so one barrier does
-        float *buf = red + ((step % 2) * wt + my_t) * cut.wk * rows * W4_ROWS;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int m = 8 * n + 2 * t + c % 2;
-                if (m < rows) buf[(my_k * rows + m) * W4_ROWS + g + c / 2 * 8] = acc[n][c];
+            if (cut.wk > 1) asm volatile("bar.sync %0, %1;" ::"r"(my_t + 1), "r"(cut.wk * 32) : "memory");
+            else __syncwarp();
+            if (cut.wk == 1 && cut.split > 1) continue;
+            buf -= my_k * tile_floats;
+#pragma unroll 1
+            for (int e = my_k * 32 + lane; e < tile_floats; e += cut.wk * 32) {
+                float v = 0.f;
+                for (int k = 0; k < cut.wk; ++k) v += buf[k * tile_floats + e];
+                const int m = m0 + e / W4_ROWS, n = tile * W4_ROWS + e % W4_ROWS;
+                if (cut.split > 1) joined[e] = v;
+                else if (n < a.N) put_out(a, xtype, otype, m, n, !XG && a.xscales ? v * a.xscales[m] : v);
             }
-        asm volatile("bar.sync %0, %1;" ::"r"(my_t + 1), "r"(cut.wk * 32) : "memory");
-        for (int e = my_k * 32 + lane; e < rows * W4_ROWS; e += cut.wk * 32) {
-            float v = 0.f;
-            for (int k = 0; k < cut.wk; ++k) v += buf[k * rows * W4_ROWS + e];
-            const int m = e / W4_ROWS, n = tile * W4_ROWS + e % W4_ROWS;
-            if (cut.split > 1) part[(step * wt + my_t) * rows * W4_ROWS + e] = v;
-            else if (n < a.N) put_out(a, otype, m0 + m, n, v);
         }
+        if (cut.split == 1) break;
+        cl.sync();
+        const int all = cut.steps * wt * tile_floats;
+#pragma unroll 1
+        for (int e = rank * W4_THREADS + threadIdx.x; e < all; e += cut.split * W4_THREADS) {
+            const int local = e / tile_floats, i = e - local * tile_floats;
+            const int at = (cluster + (batch * cut.steps + local / wt) * cut.clusters) * wt + local % wt;
+            const int m = m0 + i / W4_ROWS, n = at * W4_ROWS + i % W4_ROWS;
+            if (at >= tiles || n >= a.N) continue;
+            float v = 0.f;
+            for (int k = 0; k < cut.split; ++k) v += *cl.map_shared_rank(part + e, k);
+            put_out(a, xtype, otype, m, n, !XG && a.xscales ? v * a.xscales[m] : v);
+        }
+        cl.sync();  // no block's sums go while another reads them
     }
-    if (cut.split == 1) return;
-
-    namespace cg = cooperative_groups;
-    const cg::cluster_group cl = cg::this_cluster();
-    cl.sync();
-    const int all = cut.steps * wt * rows * W4_ROWS;
-    for (int e = rank * W4_THREADS + threadIdx.x; e < all; e += cut.split * W4_THREADS) {
-        const int local = e / (rows * W4_ROWS), i = e - local * rows * W4_ROWS;
-        const int tile = (cluster + local / wt * cut.clusters) * wt + local % wt;
-        const int m = i / W4_ROWS, n = tile * W4_ROWS + i % W4_ROWS;
-        if (n >= a.N) continue;
-        float v = 0.f;
-        for (int k = 0; k < cut.split; ++k) v += *cl.map_shared_rank(part + e, k);
-        put_out(a, otype, m0 + m, n, v);
-    }
-    cl.sync();  // no block's sums go while another reads them
 }
 
 // Blocks that the device holds at once when every `split` of them form a cluster. Looked up once per device, as the kernel
 // gets its shared memory.
-template <class X, int SUB, int NT, bool XG>
+template <int SUB, int NT, bool XG, int RING>
 int resident(int split) {
-    const auto kernel = k_gemv_w4<X, SUB, NT, XG>;
+    const auto kernel = k_gemv_w4<SUB, NT, XG, RING>;
     static std::atomic<int> known[64][4];
     int dev = 0, n = 0;
     cudaGetDevice(&dev);
@@ -338,54 +394,53 @@ int resident(int split) {
     return std::max(n, split);
 }
 
-template <class X, int SUB, int NT, bool XG>
-void launch(const W4Args &a, int mt, int otype, cudaStream_t st) {
-    const auto kernel = k_gemv_w4<X, SUB, NT, XG>;
-    const int kb = (a.K + W4_COLS - 1) / W4_COLS, tiles = (a.N + W4_ROWS - 1) / W4_ROWS, rec = w4_record_bytes(a.group);
-    W4Cut cut;
-    cut.rows = (int)((a.M + (int64_t)mt - 1) / mt);
-    cut.vec = reinterpret_cast<uintptr_t>(a.x) % (8 * sizeof(X)) == 0 && a.ldx % 8 == 0;
-    const int ring = W4_WARPS * W4_RING * rec;
-    const auto x_bytes = [&](int split) {
-        return cut.rows * ((kb + split - 1) / split * W4_COLS * 2 + X_PAD * 2);
-    };
-    const auto xsc_bytes = [&](int split) { return XG ? cut.rows * ((kb + split - 1) / split) * (W4_COLS / a.xgroup) * 4 : 0; };
-    // K is split until a block's token rows are small beside its weights, or small at all
-    const int64_t share = (int64_t)tiles * kb * rec / resident<X, SUB, NT, XG>(1);
-    const int tile_bytes = cut.rows * W4_ROWS * 4;
-    const auto fixed_bytes = [&](int split) { return ring + x_bytes(split) + xsc_bytes(split); };
-    while (cut.split < 8 && cut.split * 2 <= kb &&
-           (x_bytes(cut.split) > std::max<int64_t>(X_SMALL, share / X_PART) ||
-            fixed_bytes(cut.split) + W4_WARPS * tile_bytes > SMEM_MAX))
-        cut.split *= 2;
-    const int fixed = fixed_bytes(cut.split);
-    // Slices of the records within a block: the fewest record times, where a tile's end costs one or two of them.
-    const int most = std::max(1, resident<X, SUB, NT, XG>(cut.split) / cut.split / mt);
+// Shared memory of the ring, and of `rows` token rows with their sums and scales in one of `split` slices.
+struct Fixed {
+    int ring, x, sums, xsc;
+    int all() const { return ring + x + sums + xsc; }
+};
+Fixed fixed_bytes(int ring, int group, int rows, int kb, int split, int sub, bool xg) {
+    const int recs = (kb + split - 1) / split, groups = (rows + 7) / 8 * 8 * recs * (W4_COLS / sub) * 4;
+    return {W4_WARPS * ring * w4_record_bytes(group), rows * (recs * W4_COLS * 2 + X_PAD * 2), groups, xg ? groups : 0};
+}
+
+// The cheapest cut by a model in clock cycles: a record takes a warp 16 x 46 cycles at HBM's rate or 16 x 32 per 8 token rows
+// at mma.sync's (16 warps share an SM), a tile's end some 500, staging 2,000 and 24 bytes a cycle, a join the same again.
+// Returns its cost, or INT64_MAX where nothing fits.
+int64_t best_cut(const W4Args &a, int mt, int ring, int sub, bool xg, int split, int blocks, W4Cut &out, int &bytes) {
+    const int kb = (a.K + W4_COLS - 1) / W4_COLS, tiles = (a.N + W4_ROWS - 1) / W4_ROWS, nt = (out.rows + 7) / 8;
+    const Fixed f = fixed_bytes(ring, a.group, out.rows, kb, split, sub, xg);
+    const int tile_bytes = out.rows * W4_ROWS * 4, most = std::max(1, blocks / split / mt);
     int64_t best = INT64_MAX;
-    W4Cut found = cut;
-    for (int wk = 1; wk <= W4_WARPS && wk <= kb / cut.split; wk *= 2) {
-        const int wt = W4_WARPS / wk, red = wk > 1 ? 2 * W4_WARPS * tile_bytes : 0;
-        const int all = (tiles + wt - 1) / wt, room = SMEM_MAX - fixed - red;
-        if (room < (cut.split > 1 ? wt * tile_bytes : 0)) continue;
-        int steps = (all + most - 1) / most;
-        if (cut.split > 1) steps = std::min(steps, room / (wt * tile_bytes));
-        const int clusters = (all + steps - 1) / steps, waves = (clusters + most - 1) / most;
-        const int64_t cost = (int64_t)waves * steps * (((kb + cut.split - 1) / cut.split + wk - 1) / wk + (wk > 1 ? 2 : 1));
+    for (int wk = 1; wk <= W4_WARPS && wk <= kb / split; wk *= 2) {
+        const int wt = W4_WARPS / wk, red = wk > 1 ? 2 * W4_WARPS * tile_bytes : split > 1 ? 0 : W4_WARPS * tile_bytes;
+        const int all = (tiles + wt - 1) / wt, room = SMEM_MAX - f.all() - red, clusters = std::min(all, most);
+        int steps = (all + clusters - 1) / clusters, batches = 1;
+        if (room < (split > 1 ? wt * tile_bytes : 0)) continue;
+        if (split > 1) {
+            batches = (steps * wt * tile_bytes + room - 1) / room;
+            while ((steps + batches - 1) / batches * wt * tile_bytes > room) ++batches;
+            steps = (steps + batches - 1) / batches;
+        }
+        const int64_t count = ((kb + split - 1) / split + wk - 1) / wk;
+        int64_t cost = 2000 + f.x * (out.vec ? 1 : 3) / 24 + (int64_t)batches * steps * (count * 16 * std::max(46, 32 * nt) + 500);
+        if (split > 1) cost += batches * (2000 + (int64_t)steps * wt * tile_bytes / 24);
         if (cost >= best) continue;
         best = cost;
-        found.wk = wk;
-        found.clusters = clusters;
-        found.steps = steps;
-        found.split = cut.split;
-        found.x_at = ring;
-        found.xsc_at = ring + x_bytes(cut.split);
-        found.red_at = fixed;
-        found.part_at = fixed + red;
+        out.split = split, out.wk = wk, out.clusters = clusters, out.steps = steps, out.batches = batches;
+        out.x_at = f.ring;
+        out.sums_at = out.x_at + f.x;
+        out.xsc_at = out.sums_at + f.sums;
+        out.red_at = f.all();
+        out.part_at = f.all() + red;
+        bytes = out.part_at + (split > 1 ? steps * wt * tile_bytes : 0);
     }
-    need(best < INT64_MAX, "the token rows do not fit the shared memory");
-    cut = found;
-    const int bytes = cut.part_at + (cut.split > 1 ? cut.steps * (W4_WARPS / cut.wk) * tile_bytes : 0);
+    return best;
+}
 
+template <int SUB, int NT, bool XG, int RING>
+void launch(const W4Args &a, const W4Cut &cut, int bytes, int mt, int xtype, int otype, cudaStream_t st) {
+    resident<SUB, NT, XG, RING>(1);
     cudaLaunchConfig_t c = {};
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -397,39 +452,54 @@ void launch(const W4Args &a, int mt, int otype, cudaStream_t st) {
     c.stream = st;
     c.attrs = at;
     c.numAttrs = cut.split > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&c, kernel, a, cut, otype);
+    const cudaError_t e = cudaLaunchKernelEx(&c, k_gemv_w4<SUB, NT, XG, RING>, a, cut, xtype, otype);
     need(e == cudaSuccess, cudaGetErrorString(e));
 }
 
+// Eight records in flight per warp cover what HBM holds back while the token rows are staged; four, where the token rows
+// leave no room for more.
+template <int SUB, int NT, bool XG>
+void launch_cut(const W4Args &a, int mt, int xtype, int otype, cudaStream_t st) {
+    const int kb = (a.K + W4_COLS - 1) / W4_COLS;
+    W4Cut base, cut;
+    base.rows = (int)((a.M + (int64_t)mt - 1) / mt);
+    base.vec = reinterpret_cast<uintptr_t>(a.x) % (xtype == TCB_I8 || xtype == TCB_E4M3 ? 8 : 16) == 0 && a.ldx % 8 == 0;
+    int64_t best = INT64_MAX;
+    int bytes = 0, ring = 0;
+    for (int split = 1; split <= 8 && split <= kb; split *= 2)
+        for (int r = 8; r >= 4; r -= 4) {
+            W4Cut c = base;
+            int b = 0;
+            int64_t cost = best_cut(a, mt, r, SUB, XG, split, resident<SUB, NT, XG, 8>(split), c, b);
+            if (cost == INT64_MAX) continue;
+            if (r == 4) cost += cost / 8;
+            if (cost < best) best = cost, cut = c, bytes = b, ring = r;
+            break;
+        }
+    need(best < INT64_MAX, "the token rows do not fit the shared memory");
+    if (ring == 8) launch<SUB, NT, XG, 8>(a, cut, bytes, mt, xtype, otype, st);
+    else launch<SUB, NT, XG, 4>(a, cut, bytes, mt, xtype, otype, st);
+}
+
 // Token rows are cut into equal tiles of at most 32, and of no more than a cluster's shared memory holds.
-template <class X, int SUB, bool XG>
-void launch_n(const W4Args &a, int otype, cudaStream_t st) {
+template <int SUB, bool XG>
+void launch_n(const W4Args &a, int xtype, int otype, cudaStream_t st) {
     const int kb = (a.K + W4_COLS - 1) / W4_COLS, split = kb >= 8 ? 8 : kb >= 4 ? 4 : kb >= 2 ? 2 : 1;
-    const int row = (kb + split - 1) / split * (W4_COLS * 2 + (XG ? W4_COLS / a.xgroup * 4 : 0)) + X_PAD * 2;
-    const int room = SMEM_MAX - W4_WARPS * W4_RING * w4_record_bytes(a.group);
-    const int fit = std::min(32, room / (row + W4_WARPS * W4_ROWS * 4));  // with one step of sums
-    const int64_t mt = (a.M + fit - 1ll) / fit;
-    const int64_t rows = (a.M + mt - 1) / mt;
-    if (rows <= 8) launch<X, SUB, 1, XG>(a, (int)mt, otype, st);
-    else if (rows <= 16) launch<X, SUB, 2, XG>(a, (int)mt, otype, st);
-    else if (rows <= 24) launch<X, SUB, 3, XG>(a, (int)mt, otype, st);
-    else launch<X, SUB, 4, XG>(a, (int)mt, otype, st);
+    int fit = 32;
+    while (fit > 1 && fixed_bytes(4, a.group, fit, kb, split, SUB, XG).all() + W4_WARPS * fit * W4_ROWS * 4 > SMEM_MAX) --fit;
+    const int64_t mt = (a.M + fit - 1ll) / fit, rows = (a.M + mt - 1) / mt;
+    if (rows <= 8) launch_cut<SUB, 1, XG>(a, (int)mt, xtype, otype, st);
+    else if (rows <= 16) launch_cut<SUB, 2, XG>(a, (int)mt, xtype, otype, st);
+    else if (rows <= 24) launch_cut<SUB, 3, XG>(a, (int)mt, xtype, otype, st);
+    else launch_cut<SUB, 4, XG>(a, (int)mt, xtype, otype, st);
 }
 
-template <class X, bool XG>
-void launch_s(const W4Args &a, int otype, cudaStream_t st) {
-    const int sub = XG ? std::min(a.group, a.xgroup) : a.group;
-    if (sub == 32) launch_n<X, 32, XG>(a, otype, st);
-    else if (sub == 64) launch_n<X, 64, XG>(a, otype, st);
-    else launch_n<X, 128, XG>(a, otype, st);
-}
-
-template <class X>
-void launch_x(const W4Args &a, int otype, cudaStream_t st) {
-    if constexpr (sizeof(X) == 1) {
-        if (a.xgroup) return launch_s<X, true>(a, otype, st);
-    }
-    launch_s<X, false>(a, otype, st);
+template <bool XG>
+void launch_s(const W4Args &a, int xtype, int otype, cudaStream_t st) {
+    const int sub = a.xgroup ? std::min(a.group, a.xgroup) : a.group;
+    if (sub == 32) launch_n<32, XG>(a, xtype, otype, st);
+    else if (sub == 64) launch_n<64, XG>(a, xtype, otype, st);
+    else launch_n<128, XG>(a, xtype, otype, st);
 }
 
 }  // namespace
@@ -448,10 +518,8 @@ void launch_gemv_w4(const W4Args &a, int xtype, int otype, cudaStream_t st) {
     need(a.x && a.w && a.out, "x, w or out is NULL");
     need(reinterpret_cast<uintptr_t>(a.w) % 16 == 0, "w is not 16-byte aligned");
     need(a.res != a.out || !a.res || a.ldr == a.ldo || a.M == 1, "res is out with another pitch");
-    if (xtype == TCB_BF16) launch_x<bf16>(a, otype, st);
-    else if (xtype == TCB_F16) launch_x<f16>(a, otype, st);
-    else if (xtype == TCB_I8) launch_x<int8_t>(a, otype, st);
-    else launch_x<e4m3>(a, otype, st);
+    if (a.xgroup || xtype == TCB_BF16) launch_s<true>(a, xtype, otype, st);
+    else launch_s<false>(a, xtype, otype, st);
     check_token_launch("k_gemv_w4");
 }
 

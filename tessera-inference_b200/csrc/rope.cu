@@ -65,13 +65,13 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope(RopeArgs a, int units, in
         for (int u = threadIdx.x - rl * units; u < units; u += ROPE_THREADS) {
             if (u >= turning) {
                 const int c = a.rot + (u - turning) * V;
-                for (int h = h0; h < h1; h += 2 * ROPE_AHEAD) {
-                    Vec<T, V> b[2 * ROPE_AHEAD];
+                for (int h = h0; h < h1; h += ROPE_AHEAD) {
+                    Vec<T, V> b[ROPE_AHEAD];
 #pragma unroll
-                    for (int k = 0; k < 2 * ROPE_AHEAD; ++k)
+                    for (int k = 0; k < ROPE_AHEAD; ++k)
                         if (h + k < h1) b[k] = load<T, V>(x + (h + k) * a.hsx + c);
 #pragma unroll
-                    for (int k = 0; k < 2 * ROPE_AHEAD; ++k)
+                    for (int k = 0; k < ROPE_AHEAD; ++k)
                         if (h + k < h1) store<T, V>(o + (h + k) * a.hso + c, b[k]);
                 }
                 continue;
