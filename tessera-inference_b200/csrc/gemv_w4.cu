@@ -45,6 +45,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// the same from c, or from zero
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float4 c) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -56,6 +63,11 @@ __device__ __forceinline__ void cp_async_wait() {
 __device__ __forceinline__ uint4 lds128(uint32_t p) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 lds_f32x4(uint32_t p) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(p) : "memory");
     return v;
 }
 __device__ __forceinline__ float2 lds_f32x2(uint32_t p) {
@@ -91,12 +103,12 @@ __device__ __forceinline__ uint4 x8(const void *x, int64_t i, int64_t end, bool 
 }
 
 // How a launch cuts the work. `split` blocks of a cluster share K; within a block the warps are 16 / wk row tiles times wk
-// slices of the records. Cluster c of `clusters` takes row tiles ((c + i clusters) (16 / wk)) + 0 .. in step i; after every
-// `steps` of them, `batches` times, a cluster joins its slices' sums.
+// slices of the records. Tile j of cluster c of `clusters` in step i is row tile c + (16 / wk i + j) clusters, so that all SMs
+// get work; after every `steps` steps, `batches` times, a cluster joins its slices' sums.
 struct W4Cut {
     int split = 1, wk = 1, clusters = 1, steps = 1, batches = 1;
     int rows = 1;                                                    // token rows of a full tile
-    int x_at = 0, sums_at = 0, xsc_at = 0, red_at = 0, part_at = 0;  // byte offsets in shared memory
+    int x_at = 0, sums_at = 0, red_at = 0, part_at = 0;              // byte offsets in shared memory
     bool vec = false;                                                // x rows can be read in 8-element steps
 };
 
@@ -156,8 +168,8 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
     // records of this warp in a tile, at least one, in a row
     const int r0 = (b1 - b0) * my_k / cut.wk, count = (b1 - b0) * (my_k + 1) / cut.wk - r0;
 
-    // This slice of the token rows: 32 times 8 columns of a row per warp and pass, zero behind the last column. The first
-    // pass's loads go out before the weights', and every pass's before the one in front is worked on.
+    // This slice of the token rows: 32 times 8 columns of a row per warp and pass, zero behind the last column. The loads
+    // of a warp's first two passes go out before the weights', later ones two passes ahead of their use.
     const int pitch = (kb + cut.split - 1) / cut.split * W4_COLS + X_PAD, k0 = b0 * W4_COLS, kn = (b1 - b0) * W4_COLS;
     const int passes = (kn + 255) / 256;
     const bool wide = xtype == TCB_BF16 || xtype == TCB_F16;
@@ -167,36 +179,37 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
         if (e >= rows * passes || k >= kn) return make_uint4(0, 0, 0, 0);
         return x8(a.x, row + k0 + k, row + a.K, wide, cut.vec);
     };
-    uint4 ahead = x_load(warp);
+    uint4 ahead = x_load(warp), ahead2 = x_load(warp + W4_WARPS);
 
     // the ring: a warp's lanes copy what they read themselves, but for the scales (lanes below `tail`, 16 bytes each)
     const uint32_t ring = smem_u32(smem) + warp * RING * rec, ring_end = ring + RING * rec;
     const int tail = (rec - W4_CODE_BYTES) / 16;
-    const int first = cluster * wt + my_t, hop = cut.clusters * wt;  // tiles of this warp: first, first + hop, ...
+    const int first = cluster + my_t * cut.clusters, hop = cut.clusters * wt;  // tiles of this warp: first, first + hop, ...
     const uint8_t *f_src = static_cast<const uint8_t *>(a.w) + ((int64_t)first * kb + b0 + r0) * rec + lane * 16;
     int f_left = first < tiles ? (tiles - first + hop - 1) / hop * count : 0, f_rec = count;
-    uint32_t f_dst = ring;
-    const auto fetch = [&] {
-        if (f_left > 0) {
-            cp_async16(f_dst + lane * 16, f_src);
-            cp_async16(f_dst + 512 + lane * 16, f_src + 512);
-            if (lane < tail) cp_async16(f_dst + W4_CODE_BYTES + lane * 16, f_src + W4_CODE_BYTES);
-            --f_left;
+    const int64_t f_hop = ((int64_t)hop * kb - count) * rec;
+    const auto fetch = [&](uint32_t dst) {
+        if (--f_left >= 0) {
+            cp_async16(dst, f_src);
+            cp_async16(dst + 512, f_src + 512);
+            if (lane < tail) cp_async16(dst + W4_CODE_BYTES, f_src + W4_CODE_BYTES);
             f_src += rec;
-            if (--f_rec == 0) f_rec = count, f_src += ((int64_t)hop * kb - count) * rec;
-            f_dst = f_dst + rec == ring_end ? ring : f_dst + rec;
+            if (--f_rec == 0) f_rec = count, f_src += f_hop;
         }
         cp_async_commit();
     };
 #pragma unroll 1
-    for (int s = 0; s < RING - 1; ++s) fetch();
+    for (int s = 0; s < RING - 1; ++s) fetch(ring + s * rec + lane * 16);
 
     uint16_t *xs = reinterpret_cast<uint16_t *>(smem + cut.x_at);
-    float *sums = reinterpret_cast<float *>(smem + cut.sums_at), *xsc = reinterpret_cast<float *>(smem + cut.xsc_at);
+    // per group and pair of token rows: the pair's sums, twice (what X starts with), then its scales
+    float *sums = reinterpret_cast<float *>(smem + cut.sums_at);
+    constexpr int PAIR = XG ? 8 : 4, GROUP = 4 * NT * PAIR;
 #pragma unroll 1
     for (int e = warp; e < rows * passes; e += W4_WARPS) {
         const uint4 v = ahead;
-        ahead = x_load(e + W4_WARPS);
+        ahead = ahead2;
+        ahead2 = x_load(e + 2 * W4_WARPS);
         const int m = e / passes, k = (e - m * passes) * 256 + lane * 8;
         uint32_t w[4] = {v.x, v.y, v.z, v.w};
         float f[8], back = 1.f;
@@ -238,13 +251,13 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
 #pragma unroll
         for (int o = 1; o < SUB / 8; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
         if (k < kn) {
-            *reinterpret_cast<uint4 *>(xs + m * pitch + k) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4 *>(xs + m * pitch + k) = make_uint4(w[0], w[2], w[1], w[3]);  // X's half, then Y's
             if (k % SUB == 0) {
-                const int at = k / SUB * 8 * NT + m;
-                sums[at] = sum * (-8.f * 0x1p-24f);
+                float *at = sums + k / SUB * GROUP + m / 2 * PAIR + m % 2;
+                at[0] = at[2] = sum * (-8.f * 0x1p-24f);
                 if constexpr (XG) {
                     if (xtype != TCB_BF16) back = k0 + k < a.K ? __ldg(a.xscales + (int64_t)(m0 + m) * ((a.K + a.xgroup - 1) / a.xgroup) + (k0 + k) / a.xgroup) : 0.f;
-                    xsc[at] = back * 0x1p24f;
+                    at[4] = back * 0x1p24f;
                 }
             }
         }
@@ -254,21 +267,22 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
     uint32_t brow[NT];  // lanes behind the last token row read it again; their sums are not written
 #pragma unroll
     for (int n = 0; n < NT; ++n) brow[n] = smem_u32(xs) + (min(8 * n + g, rows - 1) * pitch + 8 * t) * 2;
-    const uint32_t my_sums = smem_u32(sums) + 8 * t, my_xsc = smem_u32(xsc) + 8 * t;
+    const uint32_t my_sums = smem_u32(sums) + PAIR * 4 * t;
     float *red = reinterpret_cast<float *>(smem + cut.red_at), *part = reinterpret_cast<float *>(smem + cut.part_at);
     const int tile_floats = rows * W4_ROWS;
     namespace cg = cooperative_groups;
     const cg::cluster_group cl = cg::this_cluster();
 
-    uint32_t slot = ring;
+    uint32_t slot = ring, before = ring + (RING - 1) * rec;
     int tile = first;
 #pragma unroll 1
     for (int batch = 0; batch < cut.batches; ++batch) {
 #pragma unroll 1
         for (int step = 0; step < cut.steps && tile < tiles; ++step, tile += hop) {  // alike for all warps of a tile
             float acc[NT][4] = {};
+            uint32_t xo = r0 * W4_COLS * 2, so = my_sums + r0 * (W4_COLS / SUB) * GROUP * 4;
 #pragma unroll 1
-            for (int r = r0; r < r0 + count; ++r) {
+            for (int r = 0; r < count; ++r) {
                 cp_async_wait<RING - 2>();
                 __syncwarp();
                 const uint4 lo = lds128(slot + lane * 16), hi = lds128(slot + 512 + lane * 16);
@@ -279,37 +293,34 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
                     su[j] = lds_bf16(p);
                     sv[j] = lds_bf16(p + 16);
                 }
-                fetch();  // into the slot read in the round before
+                fetch(before + lane * 16);  // the slot read in the round before
+                before = slot;
                 slot = slot + rec == ring_end ? ring : slot + rec;
                 const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
                 float X[NT][4], Y[NT][4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int sub = j * 32 / SUB;
-                    if (j * 32 % SUB == 0) {
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            const float2 s = lds_f32x2(my_sums + ((r * (W4_COLS / SUB) + sub) * 8 * NT + 8 * n) * 4);
-                            X[n][0] = X[n][2] = s.x;
-                            X[n][1] = X[n][3] = s.y;
-                            Y[n][0] = Y[n][1] = Y[n][2] = Y[n][3] = 0.f;
-                        }
-                    }
                     const uint32_t vl = wl[j] >> 8, vh = wh[j] >> 8;
                     const uint32_t A[4] = {wl[j] & 0x000f000fu, wh[j] & 0x000f000fu, vl & 0x000f000fu, vh & 0x000f000fu};
                     const uint32_t B[4] = {wl[j] & 0x00f000f0u, wh[j] & 0x00f000f0u, vl & 0x00f000f0u, vh & 0x00f000f0u};
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        const uint4 b = lds128(brow[n] + (r * W4_COLS + 32 * j) * 2);
-                        mma16816(X[n], A, b.x, b.z);
-                        mma16816(Y[n], B, b.y, b.w);
+                        const uint4 b = lds128(brow[n] + xo + 64 * j);
+                        if (j * 32 % SUB == 0) {
+                            mma16816(X[n], A, b.x, b.y, lds_f32x4(so + (sub * GROUP + 4 * n * PAIR) * 4));
+                            mma16816(Y[n], B, b.z, b.w, make_float4(0.f, 0.f, 0.f, 0.f));
+                        } else {
+                            mma16816(X[n], A, b.x, b.y);
+                            mma16816(Y[n], B, b.z, b.w);
+                        }
                     }
                     if ((j + 1) * 32 % SUB == 0) {
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             float s0 = su[sub], s1 = su[sub], s2 = sv[sub], s3 = sv[sub];
                             if constexpr (XG) {
-                                const float2 xf = lds_f32x2(my_xsc + ((r * (W4_COLS / SUB) + sub) * 8 * NT + 8 * n) * 4);
+                                const float2 xf = lds_f32x2(so + (sub * GROUP + 4 * n * PAIR + 4) * 4);
                                 s0 *= xf.x, s1 *= xf.y, s2 *= xf.x, s3 *= xf.y;
                             }
                             acc[n][0] = fmaf(fmaf(Y[n][0], 0.0625f, X[n][0]), s0, acc[n][0]);
@@ -319,6 +330,8 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
                         }
                     }
                 }
+                xo += W4_COLS * 2;
+                so += W4_COLS / SUB * GROUP * 4;
             }
             // Slices' sums meet in shared memory, in slice order. Two buffers in turn, so one barrier does; a warp that has
             // its tile alone needs one buffer, or none when the cluster joins slices anyway.
@@ -352,7 +365,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
 #pragma unroll 1
         for (int e = rank * W4_THREADS + threadIdx.x; e < all; e += cut.split * W4_THREADS) {
             const int local = e / tile_floats, i = e - local * tile_floats;
-            const int at = (cluster + (batch * cut.steps + local / wt) * cut.clusters) * wt + local % wt;
+            const int at = cluster + (batch * cut.steps * wt + local) * cut.clusters;
             const int m = m0 + i / W4_ROWS, n = at * W4_ROWS + i % W4_ROWS;
             if (at >= tiles || n >= a.N) continue;
             float v = 0.f;
@@ -396,16 +409,17 @@ int resident(int split) {
 
 // Shared memory of the ring, and of `rows` token rows with their sums and scales in one of `split` slices.
 struct Fixed {
-    int ring, x, sums, xsc;
-    int all() const { return ring + x + sums + xsc; }
+    int ring, x, sums;
+    int all() const { return ring + x + sums; }
 };
 Fixed fixed_bytes(int ring, int group, int rows, int kb, int split, int sub, bool xg) {
-    const int recs = (kb + split - 1) / split, groups = (rows + 7) / 8 * 8 * recs * (W4_COLS / sub) * 4;
-    return {W4_WARPS * ring * w4_record_bytes(group), rows * (recs * W4_COLS * 2 + X_PAD * 2), groups, xg ? groups : 0};
+    const int recs = (kb + split - 1) / split, pairs = (rows + 7) / 8 * 4;
+    return {W4_WARPS * ring * w4_record_bytes(group), rows * (recs * W4_COLS * 2 + X_PAD * 2),
+            pairs * recs * (W4_COLS / sub) * (xg ? 32 : 16)};
 }
 
-// The cheapest cut by a model in clock cycles: a record takes a warp 16 x 46 cycles at HBM's rate or 16 x 32 per 8 token rows
-// at mma.sync's (16 warps share an SM), a tile's end some 500, staging 2,000 and 24 bytes a cycle, a join the same again.
+// The cheapest cut by a model in clock cycles: a record takes an SM 46 cycles at HBM's rate or 32 per 8 token rows at
+// mma.sync's, and a warp 400 at least; a tile's end some 500, staging 2,000 and 24 bytes a cycle, a join the same again.
 // Returns its cost, or INT64_MAX where nothing fits.
 int64_t best_cut(const W4Args &a, int mt, int ring, int sub, bool xg, int split, int blocks, W4Cut &out, int &bytes) {
     const int kb = (a.K + W4_COLS - 1) / W4_COLS, tiles = (a.N + W4_ROWS - 1) / W4_ROWS, nt = (out.rows + 7) / 8;
@@ -414,8 +428,8 @@ int64_t best_cut(const W4Args &a, int mt, int ring, int sub, bool xg, int split,
     int64_t best = INT64_MAX;
     for (int wk = 1; wk <= W4_WARPS && wk <= kb / split; wk *= 2) {
         const int wt = W4_WARPS / wk, red = wk > 1 ? 2 * W4_WARPS * tile_bytes : split > 1 ? 0 : W4_WARPS * tile_bytes;
-        const int all = (tiles + wt - 1) / wt, room = SMEM_MAX - f.all() - red, clusters = std::min(all, most);
-        int steps = (all + clusters - 1) / clusters, batches = 1;
+        const int room = SMEM_MAX - f.all() - red, clusters = std::min(tiles, most), each = (tiles + clusters - 1) / clusters;
+        int steps = (each + wt - 1) / wt, batches = 1;
         if (room < (split > 1 ? wt * tile_bytes : 0)) continue;
         if (split > 1) {
             batches = (steps * wt * tile_bytes + room - 1) / room;
@@ -423,14 +437,14 @@ int64_t best_cut(const W4Args &a, int mt, int ring, int sub, bool xg, int split,
             steps = (steps + batches - 1) / batches;
         }
         const int64_t count = ((kb + split - 1) / split + wk - 1) / wk;
-        int64_t cost = 2000 + f.x * (out.vec ? 1 : 3) / 24 + (int64_t)batches * steps * (count * 16 * std::max(46, 32 * nt) + 500);
+        int64_t cost = std::max((int64_t)each * ((kb + split - 1) / split) * std::max(46, 32 * nt), batches * steps * count * 400);
+        cost += 2000 + f.x * (out.vec ? 1 : 3) / 24 + batches * steps * 500;
         if (split > 1) cost += batches * (2000 + (int64_t)steps * wt * tile_bytes / 24);
         if (cost >= best) continue;
         best = cost;
         out.split = split, out.wk = wk, out.clusters = clusters, out.steps = steps, out.batches = batches;
         out.x_at = f.ring;
         out.sums_at = out.x_at + f.x;
-        out.xsc_at = out.sums_at + f.sums;
         out.red_at = f.all();
         out.part_at = f.all() + red;
         bytes = out.part_at + (split > 1 ? steps * wt * tile_bytes : 0);
