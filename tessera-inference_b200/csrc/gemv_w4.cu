@@ -81,24 +81,21 @@ __device__ __forceinline__ float lds_bf16(uint32_t p) {
     return bf16lo(v);
 }
 
-// 8 elements of x from element i on, as they are stored: 16-bit ones fill four words, 8-bit ones two. Elements from `end` on
-// are zero; `vec`: i is a multiple of 8 and rows start at 8-element boundaries.
-__device__ __forceinline__ uint4 x8(const void *x, int64_t i, int64_t end, bool wide, bool vec) {
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (vec && i + 8 <= end) {
+// 8 elements of x from element i on, a multiple of 8, as they are stored: 16-bit ones fill four words, 8-bit ones two.
+// Elements from `end` on are zero.
+__device__ __forceinline__ uint4 x8(const void *x, int64_t i, int64_t end, bool wide) {
+    if (i + 8 <= end) {
         if (wide) return *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(x) + i);
         const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(x) + i);
         return make_uint4(q.x, q.y, 0, 0);
     }
-    if (wide) {
+    uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (i + j < end) w[j / 2] |= (uint32_t)static_cast<const uint16_t *>(x)[i + j] << 16 * (j % 2);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (i + j < end) w[j / 4] |= (uint32_t)static_cast<const uint8_t *>(x)[i + j] << 8 * (j % 4);
-    }
+    for (int j = 0; j < 8; ++j)
+        if (i + j < end) {
+            if (wide) w[j / 2] |= (uint32_t)static_cast<const uint16_t *>(x)[i + j] << 16 * (j % 2);
+            else w[j / 4] |= (uint32_t)static_cast<const uint8_t *>(x)[i + j] << 8 * (j % 4);
+        }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -168,19 +165,6 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
     // records of this warp in a tile, at least one, in a row
     const int r0 = (b1 - b0) * my_k / cut.wk, count = (b1 - b0) * (my_k + 1) / cut.wk - r0;
 
-    // This slice of the token rows: 32 times 8 columns of a row per warp and pass, zero behind the last column. The loads
-    // of a warp's first two passes go out before the weights', later ones two passes ahead of their use.
-    const int pitch = (kb + cut.split - 1) / cut.split * W4_COLS + X_PAD, k0 = b0 * W4_COLS, kn = (b1 - b0) * W4_COLS;
-    const int passes = (kn + 255) / 256;
-    const bool wide = xtype == TCB_BF16 || xtype == TCB_F16;
-    const auto x_load = [&](int e) {
-        const int m = e / passes, k = (e - m * passes) * 256 + lane * 8;
-        const int64_t row = (int64_t)(m0 + m) * a.ldx;
-        if (e >= rows * passes || k >= kn) return make_uint4(0, 0, 0, 0);
-        return x8(a.x, row + k0 + k, row + a.K, wide, cut.vec);
-    };
-    uint4 ahead = x_load(warp), ahead2 = x_load(warp + W4_WARPS);
-
     // the ring: a warp's lanes copy what they read themselves, but for the scales (lanes below `tail`, 16 bytes each)
     const uint32_t ring = smem_u32(smem) + warp * RING * rec, ring_end = ring + RING * rec;
     const int tail = (rec - W4_CODE_BYTES) / 16;
@@ -198,8 +182,40 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
         }
         cp_async_commit();
     };
+    fetch(ring + lane * 16);
+    fetch(ring + rec + lane * 16);
+
+    // This slice of the token rows: 32 times 8 columns of a row per warp and pass, zero behind the last column. Loads go out
+    // four passes ahead of their use, the first ones before most of the ring's.
+    const int pitch = (kb + cut.split - 1) / cut.split * W4_COLS + X_PAD, k0 = b0 * W4_COLS, kn = (b1 - b0) * W4_COLS;
+    const int passes = (kn + 255) / 256;
+    const bool wide = xtype == TCB_BF16 || xtype == TCB_F16;
+    // Aligned rows: columns 8 lane .. + 7 of the pass. Others: columns lane, lane + 32, ..., so that a warp's loads are
+    // consecutive; they change places in shared memory.
+    const auto x_load = [&](int e) {
+        const int m = e / passes, k = k0 + (e - m * passes) * 256;
+        const int64_t row = (int64_t)(m0 + m) * a.ldx;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (e >= rows * passes) return v;
+        if (cut.vec) {
+            if (k + lane * 8 < min(a.K, k0 + kn)) v = x8(a.x, row + k + lane * 8, row + a.K, wide);
+            return v;
+        }
+        uint32_t u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int c = k + lane + 32 * j;
+            u[j] = 0;
+            if (c < min(a.K, k0 + kn)) u[j] = wide ? static_cast<const uint16_t *>(a.x)[row + c] : static_cast<const uint8_t *>(a.x)[row + c];
+        }
+        return make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
+    };
+    uint4 ahead[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ahead[i] = x_load(warp + i * W4_WARPS);
+
 #pragma unroll 1
-    for (int s = 0; s < RING - 1; ++s) fetch(ring + s * rec + lane * 16);
+    for (int s = 2; s < RING - 1; ++s) fetch(ring + s * rec + lane * 16);
 
     uint16_t *xs = reinterpret_cast<uint16_t *>(smem + cut.x_at);
     // per group and pair of token rows: the pair's sums, twice (what X starts with), then its scales
@@ -207,10 +223,24 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
     constexpr int PAIR = XG ? 8 : 4, GROUP = 4 * NT * PAIR;
 #pragma unroll 1
     for (int e = warp; e < rows * passes; e += W4_WARPS) {
-        const uint4 v = ahead;
-        ahead = ahead2;
-        ahead2 = x_load(e + 2 * W4_WARPS);
+        uint4 v = ahead[0];
+        ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = ahead[3];
+        ahead[3] = x_load(e + 4 * W4_WARPS);
         const int m = e / passes, k = (e - m * passes) * 256 + lane * 8;
+        if (!cut.vec) {  // through the row's place in shared memory, which has the room: rows end on whole records
+            uint16_t *p = xs + m * pitch + k - lane * 7;
+            const int left = kn - (k - lane * 8);
+            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (lane + 32 * j < left) p[32 * j] = (uint16_t)(u[j / 2] >> 16 * (j % 2));
+            __syncwarp();
+            v = k < kn ? *reinterpret_cast<const uint4 *>(xs + m * pitch + k) : make_uint4(0, 0, 0, 0);
+            if (!wide)
+                v = make_uint4((v.x & 0xffu) | (v.x >> 8 & 0xff00u) | v.y << 16 & 0xff0000u | (v.y << 8 & 0xff000000u),
+                               (v.z & 0xffu) | (v.z >> 8 & 0xff00u) | v.w << 16 & 0xff0000u | (v.w << 8 & 0xff000000u), 0, 0);
+            __syncwarp();
+        }
         uint32_t w[4] = {v.x, v.y, v.z, v.w};
         float f[8], back = 1.f;
         if (xtype == TCB_BF16) {
@@ -368,8 +398,11 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
             const int at = cluster + (batch * cut.steps * wt + local) * cut.clusters;
             const int m = m0 + i / W4_ROWS, n = at * W4_ROWS + i % W4_ROWS;
             if (at >= tiles || n >= a.N) continue;
-            float v = 0.f;
-            for (int k = 0; k < cut.split; ++k) v += *cl.map_shared_rank(part + e, k);
+            float v = 0.f, u[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) u[k] = k < cut.split ? *cl.map_shared_rank(part + e, k) : 0.f;  // all on their way at once
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v += u[k];
             put_out(a, xtype, otype, m, n, !XG && a.xscales ? v * a.xscales[m] : v);
         }
         cl.sync();  // no block's sums go while another reads them
@@ -438,8 +471,8 @@ int64_t best_cut(const W4Args &a, int mt, int ring, int sub, bool xg, int split,
         }
         const int64_t count = ((kb + split - 1) / split + wk - 1) / wk;
         int64_t cost = std::max((int64_t)each * ((kb + split - 1) / split) * std::max(46, 32 * nt), batches * steps * count * 400);
-        cost += 2000 + f.x * (out.vec ? 1 : 3) / 24 + batches * steps * 500;
-        if (split > 1) cost += batches * (2000 + (int64_t)steps * wt * tile_bytes / 24);
+        cost += 2000 + f.x * (out.vec ? 1 : 2) / 24 + batches * steps * 500;
+        if (split > 1) cost += batches * (4000 + (int64_t)steps * wt * tile_bytes / 24);
         if (cost >= best) continue;
         best = cost;
         out.split = split, out.wk = wk, out.clusters = clusters, out.steps = steps, out.batches = batches;
