@@ -11,7 +11,17 @@ namespace tcb {
 namespace {
 
 constexpr int ROPE_THREADS = 256;
-constexpr int ROPE_AHEAD = 4;  // heads whose loads a thread issues together
+
+// Blocks per SM, which bound the registers, and the heads whose loads a thread issues together. Many threads with few loads
+// each hide HBM better than the reverse: on 524,288 rows of 8 heads x 160 in bf16, 6 blocks and one head (two vectors) take
+// 440 us, 4 and two heads 501, 2 and four heads 538.
+template <class T, bool INTER, int V>
+struct RopeShape {
+    static constexpr bool ONE = INTER && V > 1;  // a unit is one vector
+    static constexpr bool WIDE = sizeof(T) == 4 && V > 1;
+    static constexpr int BLOCKS = WIDE ? 5 : 6;
+    static constexpr int AHEAD = V == 1 ? 4 : (ONE ? 2 : 1) * (WIDE ? 2 : 1);
+};
 
 // cos and sin (times mscale) of pos * freq. The angle is reduced to a fraction
 // of a turn in f64, so a far position keeps its phase; the fraction is then
@@ -49,61 +59,56 @@ __device__ __forceinline__ void store(T *p, const Vec<T, V> &r) {
 }
 
 // Units of a row: first those that turn, then those that are copied (none when
-// out is x). A turning unit is two vectors of V first and V second elements of
-// the pairs (rot/2 apart), or, interleaved, two neighbouring vectors of V/2 pairs
-// each (one element each for V = 1): V pairs either way. blockIdx.y is a slice
-// of the heads.
+// out is x). A unit is the same one or two vectors of V columns in every head. Half layout: the
+// first and the second elements of V pairs, rot/2 apart. Interleaved: one vector
+// of V/2 pairs (V = 1: the two elements of a pair). blockIdx.y is a slice of the
+// heads.
 template <class T, class P, bool INTER, int V>
-__global__ void __launch_bounds__(ROPE_THREADS) k_rope(RopeArgs a, int units, int rows, int slice) {
-    const int half = a.rot / 2, turning = half / V;
+__global__ void __launch_bounds__(ROPE_THREADS, RopeShape<T, INTER, V>::BLOCKS) k_rope(const RopeArgs a, int units, int rows, int slice) {
+    constexpr bool ONE = RopeShape<T, INTER, V>::ONE;
+    constexpr int PAIRS = ONE ? V / 2 : V;  // of a unit
+    constexpr int AHEAD = RopeShape<T, INTER, V>::AHEAD;
+    const int half = a.rot / 2, turning = half / PAIRS;
     const int h0 = blockIdx.y * slice, h1 = min(a.heads, h0 + slice);
     const int rl = units < ROPE_THREADS ? threadIdx.x / units : 0;
     if (rl >= rows) return;
     for (int64_t r = (int64_t)blockIdx.x * rows + rl; r < a.M; r += (int64_t)gridDim.x * rows) {
-        const T *x = static_cast<const T *>(a.x) + r * a.ldx;
-        T *o = static_cast<T *>(a.out) + r * a.ldo;
         for (int u = threadIdx.x - rl * units; u < units; u += ROPE_THREADS) {
-            if (u >= turning) {
-                const int c = a.rot + (u - turning) * V;
-                for (int h = h0; h < h1; h += ROPE_AHEAD) {
-                    Vec<T, V> b[ROPE_AHEAD];
+            const bool turns = u < turning;
+            const int p = !turns ? a.rot + (u - turning) * V : INTER ? 2 * PAIRS * u : V * u;
+            const int second = INTER ? 1 : half;  // from a pair's first element to its second
+            float2 t[PAIRS];
+            if (turns) {
+                const double pos = (double)static_cast<const P *>(a.pos)[r * a.pos_stride];
 #pragma unroll
-                    for (int k = 0; k < ROPE_AHEAD; ++k)
-                        if (h + k < h1) b[k] = load<T, V>(x + (h + k) * a.hsx + c);
-#pragma unroll
-                    for (int k = 0; k < ROPE_AHEAD; ++k)
-                        if (h + k < h1) store<T, V>(o + (h + k) * a.hso + c, b[k]);
-                }
-                continue;
+                for (int j = 0; j < PAIRS; ++j) t[j] = turn_of(pos, a.freq[u * PAIRS + j], a.mscale, a.sign);
             }
-            const int p = INTER ? 2 * V * u : V * u, q = INTER ? p + V : p + half;
-            float2 t[V];
-            const double pos = (double)static_cast<const P *>(a.pos)[r * a.pos_stride];
+            const T *x = static_cast<const T *>(a.x) + r * a.ldx + h0 * a.hsx + p;
+            T *o = static_cast<T *>(a.out) + r * a.ldo + h0 * a.hso + p;
+            for (int h = h0; h < h1; h += AHEAD, x += AHEAD * a.hsx, o += AHEAD * a.hso) {
+                Vec<T, V> b[AHEAD], c[AHEAD];
 #pragma unroll
-            for (int j = 0; j < V; ++j) t[j] = turn_of(pos, a.freq[u * V + j], a.mscale, a.sign);
-            for (int h = h0; h < h1; h += ROPE_AHEAD) {
-                Vec<T, V> b[ROPE_AHEAD], c[ROPE_AHEAD];
-#pragma unroll
-                for (int k = 0; k < ROPE_AHEAD; ++k)
+                for (int k = 0; k < AHEAD; ++k)
                     if (h + k < h1) {
-                        b[k] = load<T, V>(x + (h + k) * a.hsx + p);
-                        c[k] = load<T, V>(x + (h + k) * a.hsx + q);
+                        b[k] = load<T, V>(x + k * a.hsx);
+                        if (!ONE && turns) c[k] = load<T, V>(x + k * a.hsx + second);
                     }
 #pragma unroll
-                for (int k = 0; k < ROPE_AHEAD; ++k) {
-                    if (h + k >= h1) break;
+                for (int k = 0; k < AHEAD; ++k)
+                    if (h + k < h1) {
+                        if (turns) {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        // pair j: element j of both vectors, or elements 2j and 2j + 1 of the two in a row
-                        T &v = INTER && V > 1 ? (2 * j < V ? b[k].v[2 * j % V] : c[k].v[2 * j % V]) : b[k].v[j];
-                        T &w = INTER && V > 1 ? (2 * j < V ? b[k].v[(2 * j + 1) % V] : c[k].v[(2 * j + 1) % V]) : c[k].v[j];
-                        const float f = to_f32(v), g = to_f32(w);
-                        v = from_f32<T>(f * t[j].x - g * t[j].y);
-                        w = from_f32<T>(f * t[j].y + g * t[j].x);
+                            for (int j = 0; j < PAIRS; ++j) {
+                                T &v = ONE ? b[k].v[2 * j % V] : b[k].v[j];
+                                T &w = ONE ? b[k].v[(2 * j + 1) % V] : c[k].v[j];
+                                const float f = to_f32(v), g = to_f32(w);
+                                v = from_f32<T>(f * t[j].x - g * t[j].y);
+                                w = from_f32<T>(f * t[j].y + g * t[j].x);
+                            }
+                            if (!ONE) store<T, V>(o + k * a.hso + second, c[k]);
+                        }
+                        store<T, V>(o + k * a.hso, b[k]);
                     }
-                    store<T, V>(o + (h + k) * a.hso + p, b[k]);
-                    store<T, V>(o + (h + k) * a.hso + q, c[k]);
-                }
             }
         }
     }
@@ -111,7 +116,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope(RopeArgs a, int units, in
 
 template <class T, class P, bool INTER, int V>
 void launch(const RopeArgs &a, cudaStream_t st) {
-    const int units = a.rot / 2 / V + (a.out == a.x ? 0 : (a.hd - a.rot) / V);
+    const int units = a.rot / (INTER && V > 1 ? V : 2 * V) + (a.out == a.x ? 0 : (a.hd - a.rot) / V);
     const int rows = std::max(1, ROPE_THREADS / units);
     const int64_t blocks = (a.M + rows - 1) / rows;
     // With few rows the heads are spread over the grid too, at the price of the angles' being computed again.
@@ -128,7 +133,7 @@ void launch_v(const RopeArgs &a, bool inter, cudaStream_t st) {
         return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % V == 0 && hs % V == 0;
     };
     // the pairs, the copied columns, and every row and head in whole vectors
-    if (a.rot / 2 % V == 0 && (a.hd - a.rot) % V == 0 && at(a.x, a.ldx, a.hsx) && at(a.out, a.ldo, a.hso)) {
+    if (a.rot % (inter ? V : 2 * V) == 0 && (a.hd - a.rot) % V == 0 && at(a.x, a.ldx, a.hsx) && at(a.out, a.ldo, a.hso)) {
         if (inter) launch<T, P, true, V>(a, st);
         else launch<T, P, false, V>(a, st);
     } else {
