@@ -17,18 +17,24 @@ void launch_rmsnorm(const RmsArgs &a, int dtype, int ytype, cudaStream_t st) {
     need(codes == (a.scales != nullptr), codes ? "scales is NULL" : "scales without 8-bit output");
     if (a.M == 0) return;
     need(a.x && a.y, "x or y is NULL");
-    // every tensor that the call uses in steps of 8 columns and 16 bytes (8 for codes)
-    const auto at = [](const void *p, int64_t ld, int bytes) {
-        return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld % RMS_UNIT == 0);
+    // Where the rows start, in elements behind a boundary of 8: the same for every tensor, or one element at a time. Groups of
+    // columns on rows of several warps need boundaries.
+    const int size = dtype == TCB_F32 ? 4 : 2;
+    const auto start = [](const void *p, int bytes) { return reinterpret_cast<uintptr_t>(p) / bytes % 8; };
+    const auto like_x = [&](const void *p, int64_t ld, int bytes) {
+        return !p || (start(p, bytes) == start(a.x, size) && (ld - a.ldx) % 8 == 0);
     };
-    const bool vec = a.D % RMS_UNIT == 0 && at(a.x, a.ldx, 16) && at(a.res, a.ldr, 16) && at(a.sum, a.lds, 16) &&
-                     at(a.y, a.ldy, codes ? 8 : 16) && at(a.g, 0, 16);
-    if (dtype == TCB_BF16) rms_launch_bf16(a, ytype, vec, st);
-    else if (dtype == TCB_F16) rms_launch_f16(a, ytype, vec, st);
-    else rms_launch_f32(a, ytype, vec, st);
+    const bool same = like_x(a.res, a.ldr, size) && like_x(a.sum, a.lds, size) && like_x(a.y, a.ldy, codes ? 1 : size);
+    const bool bounds = start(a.x, size) == 0 && a.ldx % 8 == 0;
+    RmsMode mode = SINGLE;
+    if (same && bounds && a.D % 8 == 0 && reinterpret_cast<uintptr_t>(a.g) % 16 == 0) mode = ALIGNED;
+    else if (same && (bounds || !a.group || a.D + 7 <= 32 * RMS_MAX_UNITS * RMS_UNIT)) mode = EDGED;
+    if (dtype == TCB_BF16) rms_launch_bf16(a, ytype, mode, st);
+    else if (dtype == TCB_F16) rms_launch_f16(a, ytype, mode, st);
+    else rms_launch_f32(a, ytype, mode, st);
     check_token_launch("k_rmsnorm");
 }
 
-void rms_launch_bf16(const RmsArgs &a, int ytype, bool vec, cudaStream_t st) { rms_launch_type<bf16>(a, ytype, vec, st); }
+void rms_launch_bf16(const RmsArgs &a, int ytype, RmsMode mode, cudaStream_t st) { rms_launch_type<bf16>(a, ytype, mode, st); }
 
 }  // namespace tcb

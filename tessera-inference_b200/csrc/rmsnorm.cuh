@@ -150,117 +150,110 @@ __device__ __forceinline__ Step step_of(uint32_t top_bits, float rstd) {
     return t;
 }
 
-// 8 codes from p.
+// 4 codes from q.
 template <class Y>
-__device__ __forceinline__ uint2 codes8(const float (&p)[8], const Step (&s)[8]) {
-    uint32_t w[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        float q[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = fmaf(p[4 * h + j], s[4 * h + j].hi, p[4 * h + j] * s[4 * h + j].lo);
-        if constexpr (std::is_same_v<Y, int8_t>) {
-            // adding 1.5 x 2^23 rounds to a whole number, to even, and leaves it in the low bits
-            uint32_t b[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = q[j] != q[j] ? 0u : __float_as_uint(q[j] + 12582912.f);
-            w[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-        } else {
-            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
-            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(q[2], q[3]), __NV_SATFINITE, __NV_E4M3);
-            w[h] = lo | hi << 16;
-        }
+__device__ __forceinline__ uint32_t codes4(float q0, float q1, float q2, float q3) {
+    if constexpr (std::is_same_v<Y, int8_t>) {
+        // adding 1.5 x 2^23 rounds to a whole number, to even, and leaves it in the low bits; a NaN gives 0
+        const uint32_t b0 = q0 != q0 ? 0u : __float_as_uint(q0 + 12582912.f), b1 = q1 != q1 ? 0u : __float_as_uint(q1 + 12582912.f);
+        const uint32_t b2 = q2 != q2 ? 0u : __float_as_uint(q2 + 12582912.f), b3 = q3 != q3 ? 0u : __float_as_uint(q3 + 12582912.f);
+        return __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
+    } else {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(q0, q1), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(q2, q3), __NV_SATFINITE, __NV_E4M3);
+        return __byte_perm(lo, hi, 0x5410);
     }
-    return make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ float coded(float p, const Step &s) { return fmaf(p, s.hi, p * s.lo); }
+template <class Y>
+__device__ __forceinline__ uint2 codes8(const float (&p)[8], const Step &s) {
+    return make_uint2(codes4<Y>(coded(p[0], s), coded(p[1], s), coded(p[2], s), coded(p[3], s)),
+                      codes4<Y>(coded(p[4], s), coded(p[5], s), coded(p[6], s), coded(p[7], s)));
 }
 
-// VEC: unit i of thread t is columns 8 (i TEAM + t) .. + 7, one 16-byte access
-// per 16-bit tensor. Otherwise (a pitch, pointer or width that is no multiple of
-// 8 elements) value (i, j) is column (8 i + j) TEAM + t, so that the accesses of
-// a warp are consecutive.
-template <class T, class Y, int TEAM, int NU, bool VEC>
+// How a row's columns lie on a team's threads. Unit i of thread t is 8 columns from 8 (i TEAM + t) - o on, one 16-byte access
+// per 16-bit tensor:
+//   ALIGNED  every row of every tensor starts at a 16-byte boundary and is whole units (o = 0);
+//   EDGED    the tensors' rows start equally far (o elements) behind such boundaries; the first and the last unit of a row
+//            are partly outside it and go element by element;
+//   SINGLE   nothing fits: value (i, j) is column (8 i + j) TEAM + t, one element per access, consecutive over a warp.
+enum RmsMode { ALIGNED, EDGED, SINGLE };
+
+template <class T, class Y, int TEAM, int NU, RmsMode MODE>
 __global__ void __launch_bounds__(TEAM == 512 ? 512 : TEAM == 128 ? 128 : 256) k_rmsnorm(const RmsArgs a) {
     constexpr int ROWS = TEAM <= 32 ? 256 / TEAM : 1;  // rows per block and pass
     constexpr bool CODES = sizeof(Y) == 1;
     __shared__ uint32_t red[3][TEAM > 32 ? TEAM / 32 : 1];
-    __shared__ uint32_t gtop[TEAM > 32 && !VEC && CODES ? TEAM * NU * RMS_UNIT / 32 : 1];
+    __shared__ uint32_t gtop[TEAM > 32 && MODE == SINGLE && CODES ? TEAM * NU * RMS_UNIT / 32 : 1];
     const int t = threadIdx.x % TEAM, D = a.D;
-    const auto col = [&](int i, int j) { return VEC ? (i * TEAM + t) * RMS_UNIT + j : (i * RMS_UNIT + j) * TEAM + t; };
     for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.M; r0 += (int64_t)gridDim.x * ROWS) {
         if (TEAM > 32 && r0 >= gridDim.x) __syncthreads();  // the shared words of the pass before are free
         const int64_t r = r0 + (TEAM <= 32 ? threadIdx.x / TEAM : 0);
         const int Dr = TEAM <= 32 && r >= a.M ? 0 : D;  // a team behind the last row goes through the motions
-        const T *x = static_cast<const T *>(a.x) + r * a.ldx;
-        const T *res = static_cast<const T *>(a.res) + r * a.ldr;
-        T *sum = static_cast<T *>(a.sum) + r * a.lds;
-        Unit<T> h[NU];
-#pragma unroll
-        for (int i = 0; i < NU; ++i) h[i].zero();
-        if constexpr (VEC) {
-#pragma unroll
-            for (int i = 0; i < NU; ++i)
-                if (col(i, 0) < Dr) h[i].load(x + col(i, 0));
-            if (a.res) {
-                Unit<T> q[NU];
-#pragma unroll
-                for (int i = 0; i < NU; ++i)
-                    if (col(i, 0) < Dr) q[i].load(res + col(i, 0));
-#pragma unroll
-                for (int i = 0; i < NU; ++i)
-                    if (col(i, 0) < Dr) {
-                        float u[8], v[8];
-                        h[i].get(u);
-                        q[i].get(v);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) u[j] += v[j];
-                        h[i].set(u);
-                        if (a.sum) h[i].store(sum + col(i, 0));
-                    }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NU; ++i)
+        const int o = MODE == EDGED ? (int)((reinterpret_cast<uintptr_t>(a.x) / sizeof(T) + r * a.ldx) % 8) : 0;
+        const auto col = [&](int i, int j) {
+            return MODE == SINGLE ? (i * RMS_UNIT + j) * TEAM + t : (i * TEAM + t) * RMS_UNIT + j - o;
+        };
+        const auto whole = [&](int i) { return MODE == ALIGNED ? col(i, 0) < Dr : col(i, 0) >= 0 && col(i, 8) <= Dr; };
+        const auto in = [&](int i, int j) { return (MODE != EDGED || col(i, j) >= 0) && col(i, j) < Dr; };
+        // unit i of a row that starts at p, zero outside the row; and back
+        const auto get = [&](const T *p, int i) {
+            Unit<T> u;
+            u.zero();
+            if (MODE != SINGLE && whole(i)) u.load(p + col(i, 0));
+            else if (MODE != ALIGNED && (MODE == SINGLE || (col(i, 8) > 0 && col(i, 0) < Dr))) {
 #pragma unroll
                 for (int j = 0; j < RMS_UNIT; ++j)
-                    if (col(i, j) < Dr) h[i].put(j, x[col(i, j)]);
-            if (a.res) {
+                    if (in(i, j)) u.put(j, p[col(i, j)]);
+            }
+            return u;
+        };
+        const auto put = [&](T *p, int i, const Unit<T> &u) {
+            if (MODE != SINGLE && whole(i)) u.store(p + col(i, 0));
+            else if (MODE != ALIGNED) {
 #pragma unroll
-                for (int i = 0; i < NU; ++i) {
-                    Unit<T> q;
-                    q.zero();
+                for (int j = 0; j < RMS_UNIT; ++j)
+                    if (in(i, j)) p[col(i, j)] = u.at(j);
+            }
+        };
+        Unit<T> h[NU];
+        {
+            const T *x = static_cast<const T *>(a.x) + r * a.ldx;
 #pragma unroll
-                    for (int j = 0; j < RMS_UNIT; ++j)
-                        if (col(i, j) < Dr) q.put(j, res[col(i, j)]);
-                    float u[8], v[8];
-                    h[i].get(u);
-                    q.get(v);
+            for (int i = 0; i < NU; ++i) h[i] = get(x, i);
+        }
+        if (a.res) {
+            const T *res = static_cast<const T *>(a.res) + r * a.ldr;
+            T *sum = static_cast<T *>(a.sum) + r * a.lds;
+            Unit<T> q[NU];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) u[j] += v[j];
-                    h[i].set(u);
-                    if (a.sum) {
+            for (int i = 0; i < NU; ++i) q[i] = get(res, i);
 #pragma unroll
-                        for (int j = 0; j < RMS_UNIT; ++j)
-                            if (col(i, j) < Dr) sum[col(i, j)] = h[i].at(j);
-                    }
-                }
+            for (int i = 0; i < NU; ++i) {
+                float u[8], v[8];
+                h[i].get(u);
+                q[i].get(v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) u[j] += v[j];
+                h[i].set(u);
+                if (a.sum) put(sum, i, h[i]);
             }
         }
-        const auto squares = [&](float pre) {
+        const auto squares = [&] {
             float ss = 0.f;
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
                 float v[8];
                 h[i].get(v);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) ss = fmaf(v[j] * pre, v[j] * pre, ss);
+                for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
             }
             return ss;
         };
-        float ss = team_sum<TEAM>(squares(1.f), reinterpret_cast<float *>(red[0]));
-        // Finite rows whose squares leave f32's range are scaled by a power of two first. Teams that share a warp go
-        // together; one that needs nothing multiplies by 1.
-        float pre = 1.f, eps = a.eps;
-        const bool far = isinf(ss) || (ss < 0x1p-90f && eps < 0x1p-80f);
+        float ss = team_sum<TEAM>(squares(), reinterpret_cast<float *>(red[0])), eps = a.eps;
+        // Finite rows whose squares leave f32's range are scaled by a power of two first, which in bf16 and f32 rounds nothing
+        // that counts beside the row's largest value; fp16 rows never leave it. Teams that share a warp go together.
+        const bool far = !std::is_same_v<T, f16> && (isinf(ss) || (ss < 0x1p-90f && eps < 0x1p-80f));
         if (TEAM < 32 ? __any_sync(~0u, far) : far) {
             uint32_t m = 0;
 #pragma unroll
@@ -272,98 +265,120 @@ __global__ void __launch_bounds__(TEAM == 512 ? 512 : TEAM == 128 ? 128 : 256) k
             }
             if (TEAM > 32) __syncthreads();
             m = team_max<TEAM>(m, red[1]);
-            if (far && m < 0x7f800000u) pre = isinf(ss) ? 0x1p-100f : 0x1p100f;
-            eps = eps * pre * pre;
+            if (far && m < 0x7f800000u) {
+                const float pre = isinf(ss) ? 0x1p-100f : 0x1p100f;
+                eps = eps * pre * pre;
+#pragma unroll
+                for (int i = 0; i < NU; ++i) {
+                    float v[8];
+                    h[i].get(v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] *= pre;
+                    h[i].set(v);
+                }
+            }
             if (TEAM > 32) __syncthreads();
-            ss = team_sum<TEAM>(squares(pre), reinterpret_cast<float *>(red[0]));
+            ss = team_sum<TEAM>(squares(), reinterpret_cast<float *>(red[0]));
             if (TEAM > 32) __syncthreads();
         }
         const float rstd = 1.f / sqrtf(ss / (float)D + eps);
-        Y *y = static_cast<Y *>(a.y) + r * a.ldy;
-        // the weights of a unit's columns; 1 where there are none
-        const auto weights = [&](int i, float (&g)[8]) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) g[j] = 1.f;
+        // v = h g, the weights being 1 where there are none
+        const auto weighted = [&](int i, float (&v)[8]) {
+            h[i].get(v);
             if (!a.g) return;
-            if constexpr (VEC) {
+            if constexpr (MODE == ALIGNED) {
                 if (col(i, 0) < D) {
                     const float4 u = __ldg(reinterpret_cast<const float4 *>(a.g + col(i, 0)));
-                    const float4 v = __ldg(reinterpret_cast<const float4 *>(a.g + col(i, 0)) + 1);
-                    g[0] = u.x, g[1] = u.y, g[2] = u.z, g[3] = u.w, g[4] = v.x, g[5] = v.y, g[6] = v.z, g[7] = v.w;
+                    const float4 w = __ldg(reinterpret_cast<const float4 *>(a.g + col(i, 0)) + 1);
+                    v[0] *= u.x, v[1] *= u.y, v[2] *= u.z, v[3] *= u.w, v[4] *= w.x, v[5] *= w.y, v[6] *= w.z, v[7] *= w.w;
                 }
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (col(i, j) < D) g[j] = __ldg(a.g + col(i, j));
+                    if (in(i, j)) v[j] *= __ldg(a.g + col(i, j));
             }
         };
+        Y *y = static_cast<Y *>(a.y) + r * a.ldy;
         if constexpr (!CODES) {
-            const float k = pre * rstd;
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
-                float g[8], v[8];
-                weights(i, g);
-                h[i].get(v);
+                float v[8];
+                weighted(i, v);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = (pre == 1.f ? v[j] * k : v[j] * pre * rstd) * g[j];
-                Unit<T> o;
-                o.set(v);
-                if constexpr (VEC) {
-                    if (col(i, 0) < Dr) o.store(y + col(i, 0));
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (col(i, j) < Dr) y[col(i, j)] = o.at(j);
-                }
+                for (int j = 0; j < 8; ++j) v[j] *= rstd;
+                Unit<T> u;
+                u.set(v);
+                put(y, i, u);
             }
         } else {
             float p[NU][8];
 #pragma unroll
-            for (int i = 0; i < NU; ++i) {
-                float g[8];
-                weights(i, g);
-                h[i].get(p[i]);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) p[i][j] = p[i][j] * pre * g[j];
-            }
+            for (int i = 0; i < NU; ++i) weighted(i, p[i]);
             const int ng = a.group ? (D + a.group - 1) / a.group : 1;
             float *scales = a.scales + r * ng;
-            const auto put = [&](int i, const Step (&s)[8]) {
-                const uint2 q = codes8<Y>(p[i], s);
-                if constexpr (VEC) {
-                    if (col(i, 0) < Dr) *reinterpret_cast<uint2 *>(y + col(i, 0)) = q;
-                } else {
+            const auto top_of = [&](int i) {
+                float m = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(p[i][j]));
+                return magnitude(m);
+            };
+            const auto write = [&](int i, uint2 q) {
+                if (MODE != SINGLE && whole(i)) *reinterpret_cast<uint2 *>(y + col(i, 0)) = q;
+                else if (MODE != ALIGNED) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        if (col(i, j) < Dr) reinterpret_cast<uint8_t *>(y)[col(i, j)] = (uint8_t)((j < 4 ? q.x : q.y) >> 8 * (j % 4));
+                        if (in(i, j)) reinterpret_cast<uint8_t *>(y)[col(i, j)] = (uint8_t)((j < 4 ? q.x : q.y) >> 8 * (j % 4));
                 }
             };
-            const auto fill = [](Step (&s)[8], const Step &v) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) s[j] = v;
-            };
-            Step s[8];
             if (a.group == 0) {
                 uint32_t m = 0;
 #pragma unroll
-                for (int i = 0; i < NU; ++i)
+                for (int i = 0; i < NU; ++i) m = max(m, top_of(i));
+                const Step s = step_of<Y>(team_max<TEAM>(m, red[2]), rstd);
+                if (t == 0 && Dr) scales[0] = s.s;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) m = max(m, magnitude(p[i][j]));
-                fill(s, step_of<Y>(team_max<TEAM>(m, red[2]), rstd));
-                if (t == 0 && Dr) scales[0] = s[0].s;
-#pragma unroll
-                for (int i = 0; i < NU; ++i) put(i, s);
-            } else if constexpr (VEC) {
-                // a group is 4, 8 or 16 neighbouring lanes, or the team
+                for (int i = 0; i < NU; ++i) write(i, codes8<Y>(p[i], s));
+            } else if constexpr (MODE == ALIGNED || (MODE == EDGED && TEAM > 32)) {
+                // a group is 4, 8 or 16 neighbouring lanes, or the team (o = 0 here)
                 const int lanes = min(a.group / RMS_UNIT, TEAM);
 #pragma unroll
                 for (int i = 0; i < NU; ++i) {
-                    uint32_t m = 0;
+                    const Step s = step_of<Y>(lanes_max(top_of(i), lanes), rstd);
+                    if (t % lanes == 0 && col(i, 0) < Dr) scales[col(i, 0) / a.group] = s.s;
+                    write(i, codes8<Y>(p[i], s));
+                }
+            } else if constexpr (MODE == EDGED) {
+                // The same, o columns late: values j >= o of a unit belong to the 8 columns that o = 0 would give this lane,
+                // values j < o to the lane in front.
+                const int lanes = min(a.group / RMS_UNIT, TEAM);
+                uint32_t own[NU], front[NU];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) m = max(m, magnitude(p[i][j]));
-                    fill(s, step_of<Y>(lanes_max(m, lanes), rstd));
-                    if (t % lanes == 0 && col(i, 0) < Dr) scales[col(i, 0) / a.group] = s[0].s;
-                    put(i, s);
+                for (int i = 0; i < NU; ++i) {
+                    own[i] = front[i] = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) (j < o ? front[i] : own[i]) = max(j < o ? front[i] : own[i], magnitude(p[i][j]));
+                }
+                Step before = {0.f, 0.f, 0.f};  // of the last lane's group, one unit back
+#pragma unroll
+                for (int i = 0; i < NU; ++i) {
+                    uint32_t next = __shfl_down_sync(~0u, front[i], 1, TEAM);
+                    if (i + 1 < NU) {
+                        const uint32_t wrap = __shfl_sync(~0u, front[(i + 1) % NU], 0, TEAM);
+                        if (t == TEAM - 1) next = wrap;
+                    } else if (t == TEAM - 1) next = 0;
+                    const Step s = step_of<Y>(lanes_max(max(own[i], next), lanes), rstd);
+                    const int at = col(i, 0) + o;
+                    if (t % lanes == 0 && at < Dr) scales[at / a.group] = s.s;
+                    Step f;
+                    f.hi = __shfl_up_sync(~0u, s.hi, 1, TEAM);
+                    f.lo = __shfl_up_sync(~0u, s.lo, 1, TEAM);
+                    if (t == 0) f = before;
+                    before.hi = __shfl_sync(~0u, s.hi, TEAM - 1, TEAM);
+                    before.lo = __shfl_sync(~0u, s.lo, TEAM - 1, TEAM);
+                    float q[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) q[j] = fmaf(p[i][j], j < o ? f.hi : s.hi, p[i][j] * (j < o ? f.lo : s.lo));
+                    write(i, make_uint2(codes4<Y>(q[0], q[1], q[2], q[3]), codes4<Y>(q[4], q[5], q[6], q[7])));
                 }
             } else if constexpr (TEAM <= 32) {
                 // a group is one or more neighbouring values j of all the team
@@ -374,20 +389,23 @@ __global__ void __launch_bounds__(TEAM == 512 ? 512 : TEAM == 128 ? 128 : 256) k
 #pragma unroll
                     for (int j = 0; j < 8; ++j) m[j] = magnitude(p[i][j]);
 #pragma unroll
-                    for (int o = 1; o < 8; o <<= 1)
-                        if (o < values) {
+                    for (int k = 1; k < 8; k <<= 1)
+                        if (k < values) {
 #pragma unroll
                             for (int j = 0; j < 8; ++j)
-                                if (!(j & o)) m[j] = m[j | o] = max(m[j], m[j | o]);
+                                if (!(j & k)) m[j] = m[j | k] = max(m[j], m[j | k]);
                         }
+                    Step s;
+                    float q[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         if (j % min(values, 8) == 0) {
-                            s[j] = step_of<Y>(lanes_max(m[j], TEAM), rstd);
-                            if (t == 0 && col(i, j) < Dr) scales[col(i, j) / a.group] = s[j].s;
-                        } else s[j] = s[j - 1];
+                            s = step_of<Y>(lanes_max(m[j], TEAM), rstd);
+                            if (t == 0 && col(i, j) < Dr) scales[col(i, j) / a.group] = s.s;
+                        }
+                        q[j] = coded(p[i][j], s);
                     }
-                    put(i, s);
+                    write(i, make_uint2(codes4<Y>(q[0], q[1], q[2], q[3]), codes4<Y>(q[4], q[5], q[6], q[7])));
                 }
             } else {
                 // a group is one to four neighbouring warps at one value j: joined in shared memory
@@ -403,51 +421,68 @@ __global__ void __launch_bounds__(TEAM == 512 ? 512 : TEAM == 128 ? 128 : 256) k
                 __syncthreads();
 #pragma unroll
                 for (int i = 0; i < NU; ++i) {
+                    float q[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const int c = min(col(i, j), D - 1);
-                        s[j] = step_of<Y>(gtop[c / a.group], rstd);
-                        if (col(i, j) < D && c % a.group == 0) scales[c / a.group] = s[j].s;
+                        const Step s = step_of<Y>(gtop[c / a.group], rstd);
+                        if (col(i, j) < D && c % a.group == 0) scales[c / a.group] = s.s;
+                        q[j] = coded(p[i][j], s);
                     }
-                    put(i, s);
+                    write(i, make_uint2(codes4<Y>(q[0], q[1], q[2], q[3]), codes4<Y>(q[4], q[5], q[6], q[7])));
                 }
             }
         }
     }
 }
 
-template <class T, class Y, int TEAM, int NU, bool VEC>
+template <class T, class Y, int TEAM, int NU, RmsMode MODE>
 void rms_launch(const RmsArgs &a, cudaStream_t st) {
     constexpr int threads = TEAM <= 32 ? 256 : TEAM, rows = TEAM <= 32 ? 256 / TEAM : 1;
-    k_rmsnorm<T, Y, TEAM, NU, VEC><<<(unsigned)std::min<int64_t>((a.M + rows - 1) / rows, 1 << 30), threads, 0, st>>>(a);
+    k_rmsnorm<T, Y, TEAM, NU, MODE><<<(unsigned)std::min<int64_t>((a.M + rows - 1) / rows, 1 << 30), threads, 0, st>>>(a);
 }
 
-// The smallest team that holds the row. Loads past the row are skipped, so a few sizes serve all widths.
-template <class T, class Y, bool VEC>
+// The smallest team that holds the row (and up to 7 columns in front of it). Loads outside the row are skipped, so a few
+// sizes serve all widths.
+template <class T, class Y, RmsMode MODE>
 void rms_launch_team(const RmsArgs &a, cudaStream_t st) {
-    const int units = (a.D + RMS_UNIT - 1) / RMS_UNIT;
-    if (units <= 2) rms_launch<T, Y, 2, 1, VEC>(a, st);
-    else if (units <= 8) rms_launch<T, Y, 8, 1, VEC>(a, st);
-    else if (units <= 32) rms_launch<T, Y, 32, 1, VEC>(a, st);
-    else if (units <= 64) rms_launch<T, Y, 32, 2, VEC>(a, st);
-    else if (units <= 96) rms_launch<T, Y, 32, 3, VEC>(a, st);
-    else if (units <= 128) rms_launch<T, Y, 32, 4, VEC>(a, st);
-    else if (units <= 256) rms_launch<T, Y, 128, 2, VEC>(a, st);
-    else if (units <= 384) rms_launch<T, Y, 128, 3, VEC>(a, st);
-    else if (units <= 512) rms_launch<T, Y, 128, 4, VEC>(a, st);
-    else if (units <= 1024) rms_launch<T, Y, 512, 2, VEC>(a, st);
-    else rms_launch<T, Y, 512, 4, VEC>(a, st);
+    const int units = (a.D + RMS_UNIT - 1 + (MODE == EDGED ? 7 : 0)) / RMS_UNIT;
+    if (units <= 2) return rms_launch<T, Y, 2, 1, MODE>(a, st);
+    if (units <= 8) return rms_launch<T, Y, 8, 1, MODE>(a, st);
+    if (units <= 32) return rms_launch<T, Y, 32, 1, MODE>(a, st);
+    if constexpr (MODE != SINGLE) {
+        if (units <= 64) return rms_launch<T, Y, 32, 2, MODE>(a, st);
+        if (units <= 96) return rms_launch<T, Y, 32, 3, MODE>(a, st);
+    }
+    if (units <= 128) return rms_launch<T, Y, 32, 4, MODE>(a, st);
+    if constexpr (MODE != SINGLE) {
+        if (units <= 256) return rms_launch<T, Y, 128, 2, MODE>(a, st);
+        if (units <= 384) return rms_launch<T, Y, 128, 3, MODE>(a, st);
+    }
+    if (units <= 512) return rms_launch<T, Y, 128, 4, MODE>(a, st);
+    if constexpr (MODE != SINGLE) {
+        if (units <= 1024) return rms_launch<T, Y, 512, 2, MODE>(a, st);
+    }
+    if (units <= 2048) return rms_launch<T, Y, 512, 4, MODE>(a, st);
+    // EDGED, 16,378 columns or more
+    rms_launch<T, Y, 512, 4, SINGLE>(a, st);
 }
 
 template <class T>
-void rms_launch_type(const RmsArgs &a, int ytype, bool vec, cudaStream_t st) {
-    if (ytype == TCB_I8) vec ? rms_launch_team<T, int8_t, true>(a, st) : rms_launch_team<T, int8_t, false>(a, st);
-    else if (ytype == TCB_E4M3) vec ? rms_launch_team<T, e4m3, true>(a, st) : rms_launch_team<T, e4m3, false>(a, st);
-    else vec ? rms_launch_team<T, T, true>(a, st) : rms_launch_team<T, T, false>(a, st);
+void rms_launch_type(const RmsArgs &a, int ytype, RmsMode mode, cudaStream_t st) {
+    const auto by_mode = [&](auto y) {
+        using Y = decltype(y);
+        if (mode == ALIGNED) rms_launch_team<T, Y, ALIGNED>(a, st);
+        else if (mode == EDGED) rms_launch_team<T, Y, EDGED>(a, st);
+        else rms_launch_team<T, Y, SINGLE>(a, st);
+    };
+    if (ytype == TCB_I8) by_mode(int8_t());
+    else if (ytype == TCB_E4M3) by_mode(e4m3());
+    else by_mode(T());
 }
 
-void rms_launch_bf16(const RmsArgs &a, int ytype, bool vec, cudaStream_t st);
-void rms_launch_f16(const RmsArgs &a, int ytype, bool vec, cudaStream_t st);
-void rms_launch_f32(const RmsArgs &a, int ytype, bool vec, cudaStream_t st);
+void rms_launch_bf16(const RmsArgs &a, int ytype, RmsMode mode, cudaStream_t st);
+void rms_launch_f16(const RmsArgs &a, int ytype, RmsMode mode, cudaStream_t st);
+void rms_launch_f32(const RmsArgs &a, int ytype, RmsMode mode, cudaStream_t st);
 
 }  // namespace tcb

@@ -3,6 +3,6 @@
 
 namespace tcb {
 
-void rms_launch_f16(const RmsArgs &a, int ytype, bool vec, cudaStream_t st) { rms_launch_type<f16>(a, ytype, vec, st); }
+void rms_launch_f16(const RmsArgs &a, int ytype, RmsMode mode, cudaStream_t st) { rms_launch_type<f16>(a, ytype, mode, st); }
 
 }  // namespace tcb

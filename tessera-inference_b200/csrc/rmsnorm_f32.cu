@@ -3,6 +3,6 @@
 
 namespace tcb {
 
-void rms_launch_f32(const RmsArgs &a, int ytype, bool vec, cudaStream_t st) { rms_launch_type<float>(a, ytype, vec, st); }
+void rms_launch_f32(const RmsArgs &a, int ytype, RmsMode mode, cudaStream_t st) { rms_launch_type<float>(a, ytype, mode, st); }
 
 }  // namespace tcb
