@@ -3,7 +3,7 @@
 
 namespace tcb {
 
-void launch_rmsnorm(const RmsArgs &a, int dtype, int ytype, cudaStream_t st) {
+void launch_rmsnorm(RmsArgs a, int dtype, int ytype, cudaStream_t st) {
     need(dtype == TCB_BF16 || dtype == TCB_F16 || dtype == TCB_F32, "dtype is not TCB_BF16, TCB_F16 or TCB_F32");
     const bool codes = ytype == TCB_I8 || ytype == TCB_E4M3;
     need(codes || ytype == dtype, "ytype is neither dtype, TCB_I8 nor TCB_E4M3");
@@ -17,6 +17,7 @@ void launch_rmsnorm(const RmsArgs &a, int dtype, int ytype, cudaStream_t st) {
     need(codes == (a.scales != nullptr), codes ? "scales is NULL" : "scales without 8-bit output");
     if (a.M == 0) return;
     need(a.x && a.y, "x or y is NULL");
+    a.inv_d = (float)(1.0 / a.D);
     // Where the rows start, in elements behind a boundary of 8: the same for every tensor, or one element at a time. Groups of
     // columns on rows of several warps need boundaries.
     const int size = dtype == TCB_F32 ? 4 : 2;

@@ -8,10 +8,9 @@
 // the smallest whose registers hold it: narrow rows share a warp, wide ones take
 // several warps.
 //
-// Codes: with p = h g, v / s = p Q / max|p| whatever the row's norm is. A code is
-// p times Q / max|p|, the latter carried to twice f32's precision, so it differs
-// from the definition's only where v / s is within a rounding or two of the middle
-// between two codes.
+// Codes: with p = h g, v / s = p Q / max|p| whatever the row's norm is, so a code
+// comes from four roundings and differs from the definition's only where v / s is
+// that near the middle between two codes.
 #pragma once
 
 #include <algorithm>
@@ -74,6 +73,18 @@ struct Unit {
             }
         }
     }
+    __device__ __forceinline__ void add(const Unit &b) {  // rounded to T once
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) * 2; ++i) {
+            if constexpr (std::is_same_v<T, bf16>) {
+                const __nv_bfloat162 v = __hadd2(*reinterpret_cast<const __nv_bfloat162 *>(&w[i]), *reinterpret_cast<const __nv_bfloat162 *>(&b.w[i]));
+                w[i] = *reinterpret_cast<const uint32_t *>(&v);
+            } else if constexpr (std::is_same_v<T, f16>) {
+                const __half2 v = __hadd2(*reinterpret_cast<const __half2 *>(&w[i]), *reinterpret_cast<const __half2 *>(&b.w[i]));
+                w[i] = *reinterpret_cast<const uint32_t *>(&v);
+            } else w[i] = __float_as_uint(__uint_as_float(w[i]) + __uint_as_float(b.w[i]));
+        }
+    }
     // one element at a time, for rows that no vector fits
     __device__ __forceinline__ void put(int j, T v) {
         if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(v);
@@ -110,65 +121,68 @@ __device__ __forceinline__ float team_sum(float v, float *red) {
     return v;
 }
 
-// Largest magnitude over `lanes` neighbouring lanes, as bits: magnitudes order like their bits, a NaN above all.
-__device__ __forceinline__ uint32_t lanes_max(uint32_t v, int lanes) {
-    if (lanes >= 32) return __reduce_max_sync(~0u, v);
-    for (int o = 1; o < lanes; o <<= 1) v = max(v, __shfl_xor_sync(~0u, v, o));
-    return v;
+// Largest magnitude over `lanes` neighbouring lanes, NaN if any is; of magnitudes, which order like their bits.
+__device__ __forceinline__ float lanes_max(float v, int lanes) {
+    uint32_t b = __float_as_uint(v);
+    if (lanes >= 32) return __uint_as_float(__reduce_max_sync(~0u, b));
+    for (int o = 1; o < lanes; o <<= 1) b = max(b, __shfl_xor_sync(~0u, b, o));
+    return __uint_as_float(b);
 }
 template <int TEAM>
-__device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t *red) {
+__device__ __forceinline__ float team_max(float v, float *red) {
     v = lanes_max(v, TEAM);
     if constexpr (TEAM > 32) {
         if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
         __syncthreads();
-        v = __reduce_max_sync(~0u, red[threadIdx.x % (TEAM / 32)]);
+        v = lanes_max(red[threadIdx.x % (TEAM / 32)], 32);
     }
     return v;
 }
 
-// What a group's codes are made with: p -> p hi + p lo, and its scale.
+__device__ __forceinline__ float rcp_approx(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// What a group's codes are made with: p -> p k, and its scale. k = Q / max|p|, with the error of the approximate reciprocal
+// taken out by one Newton step.
 struct Step {
-    float hi, lo, s;
+    float k, s;
 };
 template <class Y>
-__device__ __forceinline__ Step step_of(uint32_t top_bits, float rstd) {
+__device__ __forceinline__ Step step_of(float top, float rstd) {
     constexpr float Q = code_top<Y>(), R = 1.f / Q;
-    const float am = __uint_as_float(top_bits), vm = am * rstd, m = max_nan(vm, 1e-12f);
+    const float v = top * rstd, m = max_nan(v, 1e-12f);
     Step t;
     t.s = m * R;
     t.s = fmaf(fmaf(-t.s, Q, m), R, t.s);  // m / Q to f32's rounding
-    if (vm >= 1e-12f && am < 0x1p100f) {
-        float r;
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(am));
-        t.hi = Q * r;
-        t.lo = fmaf(-t.hi, am, Q) * r;  // what hi lacks of the quotient
-    } else {  // all but zero, far out of range, or NaN
-        t.hi = rstd / t.s;
-        t.lo = vm != vm ? vm : 0.f;
-    }
+    const float r = rcp_approx(top);
+    t.k = Q * r;
+    t.k = fmaf(fmaf(-t.k, top, Q), r, t.k);
+    if (!(v >= 1e-12f) || top > 0x1p100f) t.k = rstd / t.s;  // all but zero, NaN, or far out of range
     return t;
 }
 
-// 4 codes from q.
+// 4 codes of p.
 template <class Y>
-__device__ __forceinline__ uint32_t codes4(float q0, float q1, float q2, float q3) {
+__device__ __forceinline__ uint32_t codes4(float p0, float p1, float p2, float p3, const Step &s) {
+    const float q0 = p0 * s.k, q1 = p1 * s.k, q2 = p2 * s.k, q3 = p3 * s.k;
     if constexpr (std::is_same_v<Y, int8_t>) {
-        // adding 1.5 x 2^23 rounds to a whole number, to even, and leaves it in the low bits; a NaN gives 0
-        const uint32_t b0 = q0 != q0 ? 0u : __float_as_uint(q0 + 12582912.f), b1 = q1 != q1 ? 0u : __float_as_uint(q1 + 12582912.f);
-        const uint32_t b2 = q2 != q2 ? 0u : __float_as_uint(q2 + 12582912.f), b3 = q3 != q3 ? 0u : __float_as_uint(q3 + 12582912.f);
-        return __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
+        // adding 1.5 x 2^23 rounds to a whole number, to even, and leaves it in the low bits; a group with a NaN gives 0
+        const uint32_t b0 = __float_as_uint(q0 + 12582912.f), b1 = __float_as_uint(q1 + 12582912.f);
+        const uint32_t b2 = __float_as_uint(q2 + 12582912.f), b3 = __float_as_uint(q3 + 12582912.f);
+        const uint32_t w = __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
+        return s.s != s.s ? 0u : w;
     } else {
         const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(q0, q1), __NV_SATFINITE, __NV_E4M3);
         const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(q2, q3), __NV_SATFINITE, __NV_E4M3);
         return __byte_perm(lo, hi, 0x5410);
     }
 }
-__device__ __forceinline__ float coded(float p, const Step &s) { return fmaf(p, s.hi, p * s.lo); }
 template <class Y>
 __device__ __forceinline__ uint2 codes8(const float (&p)[8], const Step &s) {
-    return make_uint2(codes4<Y>(coded(p[0], s), coded(p[1], s), coded(p[2], s), coded(p[3], s)),
-                      codes4<Y>(coded(p[4], s), coded(p[5], s), coded(p[6], s), coded(p[7], s)));
+    return make_uint2(codes4<Y>(p[0], p[1], p[2], p[3], s), codes4<Y>(p[4], p[5], p[6], p[7], s));
 }
 
 // How a row's columns lie on a team's threads. Unit i of thread t is 8 columns from 8 (i TEAM + t) - o on, one 16-byte access
@@ -179,29 +193,45 @@ __device__ __forceinline__ uint2 codes8(const float (&p)[8], const Step &s) {
 //   SINGLE   nothing fits: value (i, j) is column (8 i + j) TEAM + t, one element per access, consecutive over a warp.
 enum RmsMode { ALIGNED, EDGED, SINGLE };
 
+// Threads of a block, and the blocks that an SM shall hold, which bounds the registers.
+template <class T, int TEAM, int NU, RmsMode MODE>
+struct RmsShape {
+    static constexpr int THREADS = TEAM <= 32 ? 128 : TEAM;
+    static constexpr int REGS = MODE == EDGED ? (NU == 1 ? 40 : NU == 2 ? 56 : NU == 3 ? 72 : 88) * (sizeof(T) == 4 ? 5 : 4) / 4
+                                : NU <= 2     ? (sizeof(T) == 4 && NU == 2 ? 56 : 40)
+                                : NU == 3     ? (sizeof(T) == 4 ? 72 : TEAM == 32 ? 48 : 64)
+                                              : (sizeof(T) == 4 ? 80 : 64);
+    static constexpr int BLOCKS = 65536 / (THREADS * REGS);
+};
+
 template <class T, class Y, int TEAM, int NU, RmsMode MODE>
-__global__ void __launch_bounds__(TEAM == 512 ? 512 : TEAM == 128 ? 128 : 256) k_rmsnorm(const RmsArgs a) {
-    constexpr int ROWS = TEAM <= 32 ? 256 / TEAM : 1;  // rows per block and pass
+__global__ void __launch_bounds__(RmsShape<T, TEAM, NU, MODE>::THREADS, RmsShape<T, TEAM, NU, MODE>::BLOCKS) k_rmsnorm(const RmsArgs a) {
+    constexpr int THREADS = RmsShape<T, TEAM, NU, MODE>::THREADS, ROWS = THREADS / TEAM;  // rows per block and pass
     constexpr bool CODES = sizeof(Y) == 1;
-    __shared__ uint32_t red[3][TEAM > 32 ? TEAM / 32 : 1];
+    // units that the choice of the team leaves whole in aligned rows (a team of 512 with 4 units starts at 8,200 columns)
+    constexpr int FULL = MODE != ALIGNED || TEAM < 32 ? 0 : TEAM == 512 ? NU / 2 : NU - 1;
+    __shared__ float red[3][TEAM > 32 ? TEAM / 32 : 1];
     __shared__ uint32_t gtop[TEAM > 32 && MODE == SINGLE && CODES ? TEAM * NU * RMS_UNIT / 32 : 1];
-    const int t = threadIdx.x % TEAM, D = a.D;
+    const int t = threadIdx.x % TEAM;
     for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.M; r0 += (int64_t)gridDim.x * ROWS) {
         if (TEAM > 32 && r0 >= gridDim.x) __syncthreads();  // the shared words of the pass before are free
-        const int64_t r = r0 + (TEAM <= 32 ? threadIdx.x / TEAM : 0);
-        const int Dr = TEAM <= 32 && r >= a.M ? 0 : D;  // a team behind the last row goes through the motions
+        const int64_t r = r0 + threadIdx.x / TEAM;
+        if (TEAM == 32 && r >= a.M) break;
+        const int D = TEAM < 32 && r >= a.M ? 0 : a.D;  // a team behind the last row that shares a warp goes through the motions
         const int o = MODE == EDGED ? (int)((reinterpret_cast<uintptr_t>(a.x) / sizeof(T) + r * a.ldx) % 8) : 0;
         const auto col = [&](int i, int j) {
             return MODE == SINGLE ? (i * RMS_UNIT + j) * TEAM + t : (i * TEAM + t) * RMS_UNIT + j - o;
         };
-        const auto whole = [&](int i) { return MODE == ALIGNED ? col(i, 0) < Dr : col(i, 0) >= 0 && col(i, 8) <= Dr; };
-        const auto in = [&](int i, int j) { return (MODE != EDGED || col(i, j) >= 0) && col(i, j) < Dr; };
+        const auto whole = [&](int i) {
+            return MODE == ALIGNED ? i < FULL || col(i, 0) < D : MODE == EDGED && col(i, 0) >= 0 && col(i, 8) <= D;
+        };
+        const auto in = [&](int i, int j) { return (MODE != EDGED || col(i, j) >= 0) && col(i, j) < D; };
         // unit i of a row that starts at p, zero outside the row; and back
         const auto get = [&](const T *p, int i) {
             Unit<T> u;
-            u.zero();
-            if (MODE != SINGLE && whole(i)) u.load(p + col(i, 0));
-            else if (MODE != ALIGNED && (MODE == SINGLE || (col(i, 8) > 0 && col(i, 0) < Dr))) {
+            if (!(MODE == ALIGNED && i < FULL)) u.zero();
+            if (whole(i)) u.load(p + col(i, 0));
+            else if (MODE == SINGLE || (MODE == EDGED && col(i, 8) > 0 && col(i, 0) < D)) {
 #pragma unroll
                 for (int j = 0; j < RMS_UNIT; ++j)
                     if (in(i, j)) u.put(j, p[col(i, j)]);
@@ -209,8 +239,8 @@ __global__ void __launch_bounds__(TEAM == 512 ? 512 : TEAM == 128 ? 128 : 256) k
             return u;
         };
         const auto put = [&](T *p, int i, const Unit<T> &u) {
-            if (MODE != SINGLE && whole(i)) u.store(p + col(i, 0));
-            else if (MODE != ALIGNED) {
+            if (whole(i)) u.store(p + col(i, 0));
+            else if (MODE == SINGLE || (MODE == EDGED && col(i, 8) > 0 && col(i, 0) < D)) {
 #pragma unroll
                 for (int j = 0; j < RMS_UNIT; ++j)
                     if (in(i, j)) p[col(i, j)] = u.at(j);
@@ -224,212 +254,240 @@ __global__ void __launch_bounds__(TEAM == 512 ? 512 : TEAM == 128 ? 128 : 256) k
         }
         if (a.res) {
             const T *res = static_cast<const T *>(a.res) + r * a.ldr;
-            T *sum = static_cast<T *>(a.sum) + r * a.lds;
             Unit<T> q[NU];
 #pragma unroll
             for (int i = 0; i < NU; ++i) q[i] = get(res, i);
+            T *sum = static_cast<T *>(a.sum) + r * a.lds;
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
-                float u[8], v[8];
-                h[i].get(u);
-                q[i].get(v);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) u[j] += v[j];
-                h[i].set(u);
+                h[i].add(q[i]);
                 if (a.sum) put(sum, i, h[i]);
             }
         }
-        const auto squares = [&] {
-            float ss = 0.f;
+        float ss = 0.f;
 #pragma unroll
-            for (int i = 0; i < NU; ++i) {
-                float v[8];
-                h[i].get(v);
+        for (int i = 0; i < NU; ++i) {
+            float v[8];
+            h[i].get(v);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+            for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+        }
+        // p = h g, the weights being 1 where there are none. Made when it is needed, so that a row waits packed for its sum;
+        // EDGED rows, whose weights come one by one, make it once.
+        const auto weigh = [&](int i, float (&p)[8]) {
+            h[i].get(p);
+            if (!a.g) return;
+            if (MODE == ALIGNED) {
+                if (whole(i)) {
+                    const float4 u = __ldg(reinterpret_cast<const float4 *>(a.g + col(i, 0)));
+                    const float4 w = __ldg(reinterpret_cast<const float4 *>(a.g + col(i, 0)) + 1);
+                    p[0] *= u.x, p[1] *= u.y, p[2] *= u.z, p[3] *= u.w, p[4] *= w.x, p[5] *= w.y, p[6] *= w.z, p[7] *= w.w;
+                }
+            } else if (whole(i)) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) p[j] *= __ldg(a.g + col(i, 0) + j);
+            } else if (MODE == SINGLE || (col(i, 8) > 0 && col(i, 0) < D)) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (in(i, j)) p[j] *= __ldg(a.g + col(i, j));
             }
-            return ss;
         };
-        float ss = team_sum<TEAM>(squares(), reinterpret_cast<float *>(red[0])), eps = a.eps;
+        constexpr bool KEEP = MODE == EDGED;
+        float kept[KEEP ? NU : 1][8];
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int i = 0; i < NU; ++i) weigh(i, kept[i]);
+        }
+        const auto weighted = [&](int i, float (&p)[8]) {
+            if constexpr (KEEP) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) p[j] = kept[i][j];
+            } else weigh(i, p);
+        };
+        ss = team_sum<TEAM>(ss, red[0]);
+        float eps = a.eps;
         // Finite rows whose squares leave f32's range are scaled by a power of two first, which in bf16 and f32 rounds nothing
         // that counts beside the row's largest value; fp16 rows never leave it. Teams that share a warp go together.
         const bool far = !std::is_same_v<T, f16> && (isinf(ss) || (ss < 0x1p-90f && eps < 0x1p-80f));
         if (TEAM < 32 ? __any_sync(~0u, far) : far) {
-            uint32_t m = 0;
+            float m = 0.f;
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
                 float v[8];
                 h[i].get(v);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) m = max(m, magnitude(v[j]));
+                for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
             }
             if (TEAM > 32) __syncthreads();
             m = team_max<TEAM>(m, red[1]);
-            if (far && m < 0x7f800000u) {
-                const float pre = isinf(ss) ? 0x1p-100f : 0x1p100f;
-                eps = eps * pre * pre;
+            const float pre = !far || !(m <= 3.4028235e38f) ? 1.f : isinf(ss) ? 0x1p-100f : 0x1p100f;
+            eps = eps * pre * pre;
+            ss = 0.f;
 #pragma unroll
-                for (int i = 0; i < NU; ++i) {
-                    float v[8];
-                    h[i].get(v);
+            for (int i = 0; i < NU; ++i) {
+                float v[8];
+                h[i].get(v);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] *= pre;
-                    h[i].set(v);
+                for (int j = 0; j < 8; ++j) {
+                    v[j] *= pre;
+                    ss = fmaf(v[j], v[j], ss);
                 }
+                h[i].set(v);
+                if constexpr (KEEP) weigh(i, kept[i]);
             }
             if (TEAM > 32) __syncthreads();
-            ss = team_sum<TEAM>(squares(), reinterpret_cast<float *>(red[0]));
+            ss = team_sum<TEAM>(ss, red[0]);
             if (TEAM > 32) __syncthreads();
         }
-        const float rstd = 1.f / sqrtf(ss / (float)D + eps);
-        // v = h g, the weights being 1 where there are none
-        const auto weighted = [&](int i, float (&v)[8]) {
-            h[i].get(v);
-            if (!a.g) return;
-            if constexpr (MODE == ALIGNED) {
-                if (col(i, 0) < D) {
-                    const float4 u = __ldg(reinterpret_cast<const float4 *>(a.g + col(i, 0)));
-                    const float4 w = __ldg(reinterpret_cast<const float4 *>(a.g + col(i, 0)) + 1);
-                    v[0] *= u.x, v[1] *= u.y, v[2] *= u.z, v[3] *= u.w, v[4] *= w.x, v[5] *= w.y, v[6] *= w.z, v[7] *= w.w;
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (in(i, j)) v[j] *= __ldg(a.g + col(i, j));
-            }
-        };
+        const float rstd = rsqrtf(fmaf(ss, a.inv_d, eps));
         Y *y = static_cast<Y *>(a.y) + r * a.ldy;
         if constexpr (!CODES) {
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
-                float v[8];
-                weighted(i, v);
+                float p[8];
+                weighted(i, p);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] *= rstd;
+                for (int j = 0; j < 8; ++j) p[j] *= rstd;
                 Unit<T> u;
-                u.set(v);
+                u.set(p);
                 put(y, i, u);
             }
         } else {
-            float p[NU][8];
-#pragma unroll
-            for (int i = 0; i < NU; ++i) weighted(i, p[i]);
-            const int ng = a.group ? (D + a.group - 1) / a.group : 1;
+            const int ng = a.group ? (a.D + a.group - 1) / a.group : 1;
             float *scales = a.scales + r * ng;
-            const auto top_of = [&](int i) {
+            const auto top_of = [](const float (&p)[8]) {
                 float m = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(p[i][j]));
-                return magnitude(m);
+                for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(p[j]));
+                return m;
             };
             const auto write = [&](int i, uint2 q) {
-                if (MODE != SINGLE && whole(i)) *reinterpret_cast<uint2 *>(y + col(i, 0)) = q;
-                else if (MODE != ALIGNED) {
+                if (whole(i)) *reinterpret_cast<uint2 *>(y + col(i, 0)) = q;
+                else if (MODE == SINGLE || (MODE == EDGED && col(i, 8) > 0 && col(i, 0) < D)) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         if (in(i, j)) reinterpret_cast<uint8_t *>(y)[col(i, j)] = (uint8_t)((j < 4 ? q.x : q.y) >> 8 * (j % 4));
                 }
             };
             if (a.group == 0) {
-                uint32_t m = 0;
+                float m = 0.f;
 #pragma unroll
-                for (int i = 0; i < NU; ++i) m = max(m, top_of(i));
+                for (int i = 0; i < NU; ++i) {
+                    float p[8];
+                    weighted(i, p);
+                    m = max_nan(m, top_of(p));
+                }
                 const Step s = step_of<Y>(team_max<TEAM>(m, red[2]), rstd);
-                if (t == 0 && Dr) scales[0] = s.s;
+                if (t == 0 && D) scales[0] = s.s;
 #pragma unroll
-                for (int i = 0; i < NU; ++i) write(i, codes8<Y>(p[i], s));
+                for (int i = 0; i < NU; ++i) {
+                    float p[8];
+                    weighted(i, p);
+                    write(i, codes8<Y>(p, s));
+                }
             } else if constexpr (MODE == ALIGNED || (MODE == EDGED && TEAM > 32)) {
                 // a group is 4, 8 or 16 neighbouring lanes, or the team (o = 0 here)
                 const int lanes = min(a.group / RMS_UNIT, TEAM);
 #pragma unroll
                 for (int i = 0; i < NU; ++i) {
-                    const Step s = step_of<Y>(lanes_max(top_of(i), lanes), rstd);
-                    if (t % lanes == 0 && col(i, 0) < Dr) scales[col(i, 0) / a.group] = s.s;
-                    write(i, codes8<Y>(p[i], s));
+                    float p[8];
+                    weighted(i, p);
+                    const Step s = step_of<Y>(lanes_max(top_of(p), lanes), rstd);
+                    if (t % lanes == 0 && col(i, 0) < D) scales[col(i, 0) / a.group] = s.s;
+                    write(i, codes8<Y>(p, s));
                 }
             } else if constexpr (MODE == EDGED) {
                 // The same, o columns late: values j >= o of a unit belong to the 8 columns that o = 0 would give this lane,
                 // values j < o to the lane in front.
                 const int lanes = min(a.group / RMS_UNIT, TEAM);
-                uint32_t own[NU], front[NU];
+                float p[NU][8], own[NU], front[NU];
+#pragma unroll
+                for (int i = 0; i < NU; ++i) weighted(i, p[i]);
 #pragma unroll
                 for (int i = 0; i < NU; ++i) {
-                    own[i] = front[i] = 0;
+                    own[i] = front[i] = 0.f;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) (j < o ? front[i] : own[i]) = max(j < o ? front[i] : own[i], magnitude(p[i][j]));
+                    for (int j = 0; j < 8; ++j) {
+                        own[i] = max_nan(own[i], j < o ? 0.f : fabsf(p[i][j]));
+                        front[i] = max_nan(front[i], j < o ? fabsf(p[i][j]) : 0.f);
+                    }
                 }
-                Step before = {0.f, 0.f, 0.f};  // of the last lane's group, one unit back
+                Step before = {0.f, 0.f};  // of the last lane's group, one unit back
 #pragma unroll
                 for (int i = 0; i < NU; ++i) {
-                    uint32_t next = __shfl_down_sync(~0u, front[i], 1, TEAM);
+                    float next = __shfl_down_sync(~0u, front[i], 1, TEAM);
                     if (i + 1 < NU) {
-                        const uint32_t wrap = __shfl_sync(~0u, front[(i + 1) % NU], 0, TEAM);
+                        const float wrap = __shfl_sync(~0u, front[(i + 1) % NU], 0, TEAM);
                         if (t == TEAM - 1) next = wrap;
-                    } else if (t == TEAM - 1) next = 0;
-                    const Step s = step_of<Y>(lanes_max(max(own[i], next), lanes), rstd);
+                    } else if (t == TEAM - 1) next = 0.f;
+                    const Step s = step_of<Y>(lanes_max(max_nan(own[i], next), lanes), rstd);
                     const int at = col(i, 0) + o;
-                    if (t % lanes == 0 && at < Dr) scales[at / a.group] = s.s;
-                    Step f;
-                    f.hi = __shfl_up_sync(~0u, s.hi, 1, TEAM);
-                    f.lo = __shfl_up_sync(~0u, s.lo, 1, TEAM);
+                    if (t % lanes == 0 && at < D) scales[at / a.group] = s.s;
+                    Step f = {__shfl_up_sync(~0u, s.k, 1, TEAM), __shfl_up_sync(~0u, s.s, 1, TEAM)};
                     if (t == 0) f = before;
-                    before.hi = __shfl_sync(~0u, s.hi, TEAM - 1, TEAM);
-                    before.lo = __shfl_sync(~0u, s.lo, TEAM - 1, TEAM);
-                    float q[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) q[j] = fmaf(p[i][j], j < o ? f.hi : s.hi, p[i][j] * (j < o ? f.lo : s.lo));
-                    write(i, make_uint2(codes4<Y>(q[0], q[1], q[2], q[3]), codes4<Y>(q[4], q[5], q[6], q[7])));
+                    before = {__shfl_sync(~0u, s.k, TEAM - 1, TEAM), __shfl_sync(~0u, s.s, TEAM - 1, TEAM)};
+                    const uint2 u = codes8<Y>(p[i], s), v = codes8<Y>(p[i], f);
+                    // the first o codes by f
+                    const uint64_t mask = o ? ~0ull >> (64 - 8 * o) : 0ull;
+                    const uint64_t w = ((uint64_t)v.y << 32 | v.x) & mask | ((uint64_t)u.y << 32 | u.x) & ~mask;
+                    write(i, make_uint2((uint32_t)w, (uint32_t)(w >> 32)));
                 }
             } else if constexpr (TEAM <= 32) {
                 // a group is one or more neighbouring values j of all the team
                 const int values = a.group / TEAM;
 #pragma unroll
                 for (int i = 0; i < NU; ++i) {
-                    uint32_t m[8];
+                    float p[8], m[8];
+                    weighted(i, p);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) m[j] = magnitude(p[i][j]);
+                    for (int j = 0; j < 8; ++j) m[j] = fabsf(p[j]);
 #pragma unroll
                     for (int k = 1; k < 8; k <<= 1)
                         if (k < values) {
 #pragma unroll
                             for (int j = 0; j < 8; ++j)
-                                if (!(j & k)) m[j] = m[j | k] = max(m[j], m[j | k]);
+                                if (!(j & k)) m[j] = m[j | k] = max_nan(m[j], m[j | k]);
                         }
                     Step s;
-                    float q[8];
+                    uint32_t w[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         if (j % min(values, 8) == 0) {
                             s = step_of<Y>(lanes_max(m[j], TEAM), rstd);
-                            if (t == 0 && col(i, j) < Dr) scales[col(i, j) / a.group] = s.s;
+                            if (t == 0 && col(i, j) < D) scales[col(i, j) / a.group] = s.s;
                         }
-                        q[j] = coded(p[i][j], s);
+                        w[j] = codes4<Y>(p[j], 0.f, 0.f, 0.f, s) & 0xff;
                     }
-                    write(i, make_uint2(codes4<Y>(q[0], q[1], q[2], q[3]), codes4<Y>(q[4], q[5], q[6], q[7])));
+                    write(i, make_uint2(w[0] | w[1] << 8 | w[2] << 16 | w[3] << 24, w[4] | w[5] << 8 | w[6] << 16 | w[7] << 24));
                 }
             } else {
                 // a group is one to four neighbouring warps at one value j: joined in shared memory
                 for (int k = t; k < ng; k += TEAM) gtop[k] = 0;
                 __syncthreads();
 #pragma unroll
-                for (int i = 0; i < NU; ++i)
+                for (int i = 0; i < NU; ++i) {
+                    float p[8];
+                    weighted(i, p);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const uint32_t w = __reduce_max_sync(~0u, magnitude(p[i][j]));
+                        const uint32_t w = __reduce_max_sync(~0u, magnitude(p[j]));
                         if (t % 32 == 0 && col(i, j) < D) atomicMax(&gtop[col(i, j) / a.group], w);
                     }
+                }
                 __syncthreads();
 #pragma unroll
                 for (int i = 0; i < NU; ++i) {
-                    float q[8];
+                    float p[8];
+                    weighted(i, p);
+                    uint32_t w[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const int c = min(col(i, j), D - 1);
-                        const Step s = step_of<Y>(gtop[c / a.group], rstd);
+                        const Step s = step_of<Y>(__uint_as_float(gtop[c / a.group]), rstd);
                         if (col(i, j) < D && c % a.group == 0) scales[c / a.group] = s.s;
-                        q[j] = coded(p[i][j], s);
+                        w[j] = codes4<Y>(p[j], 0.f, 0.f, 0.f, s) & 0xff;
                     }
-                    write(i, make_uint2(codes4<Y>(q[0], q[1], q[2], q[3]), codes4<Y>(q[4], q[5], q[6], q[7])));
+                    write(i, make_uint2(w[0] | w[1] << 8 | w[2] << 16 | w[3] << 24, w[4] | w[5] << 8 | w[6] << 16 | w[7] << 24));
                 }
             }
         }
@@ -438,7 +496,7 @@ __global__ void __launch_bounds__(TEAM == 512 ? 512 : TEAM == 128 ? 128 : 256) k
 
 template <class T, class Y, int TEAM, int NU, RmsMode MODE>
 void rms_launch(const RmsArgs &a, cudaStream_t st) {
-    constexpr int threads = TEAM <= 32 ? 256 : TEAM, rows = TEAM <= 32 ? 256 / TEAM : 1;
+    constexpr int threads = RmsShape<T, TEAM, NU, MODE>::THREADS, rows = threads / TEAM;
     k_rmsnorm<T, Y, TEAM, NU, MODE><<<(unsigned)std::min<int64_t>((a.M + rows - 1) / rows, 1 << 30), threads, 0, st>>>(a);
 }
 
@@ -456,7 +514,8 @@ void rms_launch_team(const RmsArgs &a, cudaStream_t st) {
     }
     if (units <= 128) return rms_launch<T, Y, 32, 4, MODE>(a, st);
     if constexpr (MODE != SINGLE) {
-        if (units <= 256) return rms_launch<T, Y, 128, 2, MODE>(a, st);
+        if (units <= 192) return rms_launch<T, Y, 64, 3, MODE>(a, st);
+        if (units <= 256) return rms_launch<T, Y, 64, 4, MODE>(a, st);
         if (units <= 384) return rms_launch<T, Y, 128, 3, MODE>(a, st);
     }
     if (units <= 512) return rms_launch<T, Y, 128, 4, MODE>(a, st);

@@ -15,10 +15,10 @@ struct RmsArgs {
     int64_t ldx = 0, ldr = 0, lds = 0, ldy = 0, M = 0;
     const float *g = nullptr;
     float *scales = nullptr;
-    float eps = 0.f;
-    int D = 0, group = 0;  // group 0 = the whole row
+    float eps = 0.f, inv_d = 0.f;  // inv_d = 1 / D, set by the launcher
+    int D = 0, group = 0;          // group 0 = the whole row
 };
-void launch_rmsnorm(const RmsArgs &a, int dtype, int ytype, cudaStream_t st);
+void launch_rmsnorm(RmsArgs a, int dtype, int ytype, cudaStream_t st);
 
 struct RopeArgs {
     const void *x = nullptr, *pos = nullptr;
