@@ -193,14 +193,15 @@ __device__ __forceinline__ uint2 codes8(const float (&p)[8], const Step &s) {
 //   SINGLE   nothing fits: value (i, j) is column (8 i + j) TEAM + t, one element per access, consecutive over a warp.
 enum RmsMode { ALIGNED, EDGED, SINGLE };
 
-// Threads of a block, and the blocks that an SM shall hold, which bounds the registers.
+// Threads of a block, and the registers of a thread, which bound the blocks on an SM: about what the packed row, and for
+// EDGED rows the row in f32, needs. Fewer spill, more leave HBM waiting (bf16 to e4m3, 524,288 x 640: 48 registers 396 us, 64
+// 422, 40 456; 32,768 x 2,560 with 64 threads a row: 80 registers 50 us, 96 54, 112 56).
 template <class T, int TEAM, int NU, RmsMode MODE>
 struct RmsShape {
     static constexpr int THREADS = TEAM <= 32 ? 128 : TEAM;
-    static constexpr int REGS = MODE == EDGED ? (NU == 1 ? 40 : NU == 2 ? 56 : NU == 3 ? 72 : 88) * (sizeof(T) == 4 ? 5 : 4) / 4
-                                : NU <= 2     ? (sizeof(T) == 4 && NU == 2 ? 56 : 40)
-                                : NU == 3     ? (sizeof(T) == 4 ? 72 : TEAM == 32 ? 48 : 64)
-                                              : (sizeof(T) == 4 ? 80 : 64);
+    static constexpr int PACKED = NU <= 2 ? 40 : NU == 3 ? 48 : NU == 4 ? 64 : NU == 5 ? 80 : 96;
+    static constexpr int REGS = MODE == EDGED ? (24 + 16 * NU) * (sizeof(T) == 4 ? 5 : 4) / 4
+                                : sizeof(T) == 4 && NU > 1 ? PACKED + 16 : PACKED;
     static constexpr int BLOCKS = 65536 / (THREADS * REGS);
 };
 
@@ -370,21 +371,16 @@ __global__ void __launch_bounds__(RmsShape<T, TEAM, NU, MODE>::THREADS, RmsShape
                 }
             };
             if (a.group == 0) {
-                float m = 0.f;
+                float m = 0.f, p[NU][8];
 #pragma unroll
                 for (int i = 0; i < NU; ++i) {
-                    float p[8];
-                    weighted(i, p);
-                    m = max_nan(m, top_of(p));
+                    weighted(i, p[i]);
+                    m = max_nan(m, top_of(p[i]));
                 }
                 const Step s = step_of<Y>(team_max<TEAM>(m, red[2]), rstd);
                 if (t == 0 && D) scales[0] = s.s;
 #pragma unroll
-                for (int i = 0; i < NU; ++i) {
-                    float p[8];
-                    weighted(i, p);
-                    write(i, codes8<Y>(p, s));
-                }
+                for (int i = 0; i < NU; ++i) write(i, codes8<Y>(p[i], s));
             } else if constexpr (MODE == ALIGNED || (MODE == EDGED && TEAM > 32)) {
                 // a group is 4, 8 or 16 neighbouring lanes, or the team (o = 0 here)
                 const int lanes = min(a.group / RMS_UNIT, TEAM);
@@ -516,7 +512,8 @@ void rms_launch_team(const RmsArgs &a, cudaStream_t st) {
     if constexpr (MODE != SINGLE) {
         if (units <= 192) return rms_launch<T, Y, 64, 3, MODE>(a, st);
         if (units <= 256) return rms_launch<T, Y, 64, 4, MODE>(a, st);
-        if (units <= 384) return rms_launch<T, Y, 128, 3, MODE>(a, st);
+        if (units <= 320) return rms_launch<T, Y, 64, 5, MODE>(a, st);
+        if (units <= 384) return rms_launch<T, Y, 64, 6, MODE>(a, st);
     }
     if (units <= 512) return rms_launch<T, Y, 128, 4, MODE>(a, st);
     if constexpr (MODE != SINGLE) {
