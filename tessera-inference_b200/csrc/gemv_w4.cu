@@ -99,6 +99,33 @@ __device__ __forceinline__ uint4 x8(const void *x, int64_t i, int64_t end, bool 
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// A warp's passes (256 columns of a row) of `rows` rows of x into shared memory, N passes' loads at once. `left`: columns of x
+// from its first one here on; the rest up to kn are zero.
+template <int N, class E>
+__device__ __forceinline__ void x_scatter(const E *x, int64_t ldx, int left, int kn, int rows, uint16_t *xs, int pitch) {
+    const int passes = (kn + 255) / 256, lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int e0 = threadIdx.x >> 5; e0 < rows * passes; e0 += N * W4_WARPS) {
+        uint32_t u[N][8];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = e0 + i * W4_WARPS, m = e / passes, c = (e - m * passes) * 256 + lane;
+            const E *p = x + m * ldx + c;
+            const int end = e < rows * passes ? left : 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[i][j] = c + 32 * j < end ? (uint32_t)p[32 * j] : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = e0 + i * W4_WARPS, m = e / passes, c = (e - m * passes) * 256 + lane;
+            const int end = e < rows * passes ? kn : 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + 32 * j < end) xs[m * pitch + c + 32 * j] = (uint16_t)u[i][j];
+        }
+    }
+}
+
 // How a launch cuts the work. `split` blocks of a cluster share K; within a block the warps are 16 / wk row tiles times wk
 // slices of the records. Tile j of cluster c of `clusters` in step i is row tile c + (16 / wk i + j) clusters, so that all SMs
 // get work; after every `steps` steps, `batches` times, a cluster joins its slices' sums.
@@ -190,25 +217,11 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
     const int pitch = (kb + cut.split - 1) / cut.split * W4_COLS + X_PAD, k0 = b0 * W4_COLS, kn = (b1 - b0) * W4_COLS;
     const int passes = (kn + 255) / 256;
     const bool wide = xtype == TCB_BF16 || xtype == TCB_F16;
-    // Aligned rows: columns 8 lane .. + 7 of the pass. Others: columns lane, lane + 32, ..., so that a warp's loads are
-    // consecutive; they change places in shared memory.
     const auto x_load = [&](int e) {
-        const int m = e / passes, k = k0 + (e - m * passes) * 256;
+        const int m = e / passes, k = k0 + (e - m * passes) * 256 + lane * 8;
         const int64_t row = (int64_t)(m0 + m) * a.ldx;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (e >= rows * passes) return v;
-        if (cut.vec) {
-            if (k + lane * 8 < min(a.K, k0 + kn)) v = x8(a.x, row + k + lane * 8, row + a.K, wide);
-            return v;
-        }
-        uint32_t u[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int c = k + lane + 32 * j;
-            u[j] = 0;
-            if (c < min(a.K, k0 + kn)) u[j] = wide ? static_cast<const uint16_t *>(a.x)[row + c] : static_cast<const uint8_t *>(a.x)[row + c];
-        }
-        return make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
+        if (!cut.vec || e >= rows * passes || k >= min(a.K, k0 + kn)) return make_uint4(0, 0, 0, 0);
+        return x8(a.x, row + k, row + a.K, wide);
     };
     uint4 ahead[4];
 #pragma unroll
@@ -221,25 +234,23 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
     // per group and pair of token rows: the pair's sums, twice (what X starts with), then its scales
     float *sums = reinterpret_cast<float *>(smem + cut.sums_at);
     constexpr int PAIR = XG ? 8 : 4, GROUP = 4 * NT * PAIR;
+    if (!cut.vec) {
+        // rows that no vector fits: one element per access, consecutive over the warp, to their places first (8-bit ones as 16)
+        if (wide) x_scatter<4>(static_cast<const uint16_t *>(a.x) + (int64_t)m0 * a.ldx + k0, a.ldx, a.K - k0, kn, rows, xs, pitch);
+        else x_scatter<4>(static_cast<const uint8_t *>(a.x) + (int64_t)m0 * a.ldx + k0, a.ldx, a.K - k0, kn, rows, xs, pitch);
+        __syncwarp();
+    }
 #pragma unroll 1
     for (int e = warp; e < rows * passes; e += W4_WARPS) {
         uint4 v = ahead[0];
         ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = ahead[3];
         ahead[3] = x_load(e + 4 * W4_WARPS);
         const int m = e / passes, k = (e - m * passes) * 256 + lane * 8;
-        if (!cut.vec) {  // through the row's place in shared memory, which has the room: rows end on whole records
-            uint16_t *p = xs + m * pitch + k - lane * 7;
-            const int left = kn - (k - lane * 8);
-            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (lane + 32 * j < left) p[32 * j] = (uint16_t)(u[j / 2] >> 16 * (j % 2));
-            __syncwarp();
+        if (!cut.vec) {
             v = k < kn ? *reinterpret_cast<const uint4 *>(xs + m * pitch + k) : make_uint4(0, 0, 0, 0);
             if (!wide)
                 v = make_uint4((v.x & 0xffu) | (v.x >> 8 & 0xff00u) | v.y << 16 & 0xff0000u | (v.y << 8 & 0xff000000u),
                                (v.z & 0xffu) | (v.z >> 8 & 0xff00u) | v.w << 16 & 0xff0000u | (v.w << 8 & 0xff000000u), 0, 0);
-            __syncwarp();
         }
         uint32_t w[4] = {v.x, v.y, v.z, v.w};
         float f[8], back = 1.f;
