@@ -99,29 +99,40 @@ __device__ __forceinline__ uint4 x8(const void *x, int64_t i, int64_t end, bool 
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A warp's passes (256 columns of a row) of `rows` rows of x into shared memory, N passes' loads at once. `left`: columns of x
+// A pass is 256 columns of a token row; a warp takes every 16th of a block's.
+struct Pass {
+    int m, p, passes, dm, dp;
+    __device__ __forceinline__ Pass(int passes, int first)
+        : m(first / passes), p(first % passes), passes(passes), dm(W4_WARPS / passes), dp(W4_WARPS % passes) {}
+    __device__ __forceinline__ void next() {
+        m += dm;
+        p += dp;
+        if (p >= passes) p -= passes, ++m;
+    }
+};
+
+// A warp's passes of `rows` rows of x into shared memory, N passes' loads at once. `left`: columns of x
 // from its first one here on; the rest up to kn are zero.
 template <int N, class E>
 __device__ __forceinline__ void x_scatter(const E *x, int64_t ldx, int left, int kn, int rows, uint16_t *xs, int pitch) {
-    const int passes = (kn + 255) / 256, lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31;
+    Pass load((kn + 255) / 256, threadIdx.x >> 5), put = load;
 #pragma unroll 1
-    for (int e0 = threadIdx.x >> 5; e0 < rows * passes; e0 += N * W4_WARPS) {
+    while (load.m < rows) {
         uint32_t u[N][8];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int e = e0 + i * W4_WARPS, m = e / passes, c = (e - m * passes) * 256 + lane;
-            const E *p = x + m * ldx + c;
-            const int end = e < rows * passes ? left : 0;
+        for (int i = 0; i < N; ++i, load.next()) {
+            const int c = load.p * 256 + lane, end = load.m < rows ? left : 0;
+            const E *p = x + load.m * ldx + c;
 #pragma unroll
             for (int j = 0; j < 8; ++j) u[i][j] = c + 32 * j < end ? (uint32_t)p[32 * j] : 0u;
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int e = e0 + i * W4_WARPS, m = e / passes, c = (e - m * passes) * 256 + lane;
-            const int end = e < rows * passes ? kn : 0;
+        for (int i = 0; i < N; ++i, put.next()) {
+            const int c = put.p * 256 + lane, end = put.m < rows ? kn : 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (c + 32 * j < end) xs[m * pitch + c + 32 * j] = (uint16_t)u[i][j];
+                if (c + 32 * j < end) xs[put.m * pitch + c + 32 * j] = (uint16_t)u[i][j];
         }
     }
 }
@@ -160,21 +171,32 @@ __device__ __noinline__ float w4_plain(const W4Args &a, int xtype, int64_t m, in
     return v;
 }
 
-__device__ __noinline__ void put_out(const W4Args &a, int xtype, int otype, int m, int n, float v) {
-    if (v != v) v = w4_plain(a, xtype, m, n);
-    if (a.bias) v += a.bias[n];
-    if (a.relu) v = v < 0.f ? 0.f : v;
-    const int64_t at = m * a.ldo + n, ar = m * a.ldr + n;
-    if (otype == TCB_BF16) {
-        if (a.res) v += to_f32(static_cast<const bf16 *>(a.res)[ar]);
-        static_cast<bf16 *>(a.out)[at] = from_f32<bf16>(v);
-    } else if (otype == TCB_F16) {
-        if (a.res) v += to_f32(static_cast<const f16 *>(a.res)[ar]);
-        static_cast<f16 *>(a.out)[at] = from_f32<f16>(v);
-    } else {
-        if (a.res) v += static_cast<const float *>(a.res)[ar];
-        static_cast<float *>(a.out)[at] = v;
+// What output (m, n) is made of beside its sum.
+struct Beside {
+    float scale, bias, res;
+};
+__device__ __forceinline__ Beside beside(const W4Args &a, int otype, bool row_scales, int m, int n) {
+    Beside b = {1.f, 0.f, 0.f};
+    if (row_scales) b.scale = a.xscales[m];
+    if (a.bias) b.bias = a.bias[n];
+    if (a.res) {
+        const int64_t at = m * a.ldr + n;
+        b.res = otype == TCB_BF16  ? to_f32(static_cast<const bf16 *>(a.res)[at])
+                : otype == TCB_F16 ? to_f32(static_cast<const f16 *>(a.res)[at])
+                                   : static_cast<const float *>(a.res)[at];
     }
+    return b;
+}
+__device__ __forceinline__ void put_out(const W4Args &a, int xtype, int otype, int m, int n, float v, const Beside &b) {
+    v *= b.scale;
+    if (v != v) v = w4_plain(a, xtype, m, n);
+    v += b.bias;
+    if (a.relu) v = v < 0.f ? 0.f : v;
+    if (a.res) v += b.res;
+    const int64_t at = m * a.ldo + n;
+    if (otype == TCB_BF16) static_cast<bf16 *>(a.out)[at] = from_f32<bf16>(v);
+    else if (otype == TCB_F16) static_cast<f16 *>(a.out)[at] = from_f32<f16>(v);
+    else static_cast<float *>(a.out)[at] = v;
 }
 
 // SUB: columns whose products share both scales. NT: tiles of 8 token rows. XG: x has scales that change along a row, the
@@ -217,15 +239,20 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
     const int pitch = (kb + cut.split - 1) / cut.split * W4_COLS + X_PAD, k0 = b0 * W4_COLS, kn = (b1 - b0) * W4_COLS;
     const int passes = (kn + 255) / 256;
     const bool wide = xtype == TCB_BF16 || xtype == TCB_F16;
-    const auto x_load = [&](int e) {
-        const int m = e / passes, k = k0 + (e - m * passes) * 256 + lane * 8;
-        const int64_t row = (int64_t)(m0 + m) * a.ldx;
-        if (!cut.vec || e >= rows * passes || k >= min(a.K, k0 + kn)) return make_uint4(0, 0, 0, 0);
-        return x8(a.x, row + k, row + a.K, wide);
+    Pass go(passes, warp), load(passes, warp);  // the pass at work, and the next one to load
+    const auto x_load = [&] {
+        const int k = k0 + load.p * 256 + lane * 8;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (cut.vec && load.m < rows && k < min(a.K, k0 + kn)) {
+            const int64_t row = (int64_t)(m0 + load.m) * a.ldx;
+            v = x8(a.x, row + k, row + a.K, wide);
+        }
+        load.next();
+        return v;
     };
     uint4 ahead[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ahead[i] = x_load(warp + i * W4_WARPS);
+    for (int i = 0; i < 4; ++i) ahead[i] = x_load();
 
 #pragma unroll 1
     for (int s = 2; s < RING - 1; ++s) fetch(ring + s * rec + lane * 16);
@@ -241,11 +268,11 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
         __syncwarp();
     }
 #pragma unroll 1
-    for (int e = warp; e < rows * passes; e += W4_WARPS) {
+    for (; go.m < rows; go.next()) {
         uint4 v = ahead[0];
         ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = ahead[3];
-        ahead[3] = x_load(e + 4 * W4_WARPS);
-        const int m = e / passes, k = (e - m * passes) * 256 + lane * 8;
+        ahead[3] = x_load();
+        const int m = go.m, k = go.p * 256 + lane * 8;
         if (!cut.vec) {
             v = k < kn ? *reinterpret_cast<const uint4 *>(xs + m * pitch + k) : make_uint4(0, 0, 0, 0);
             if (!wide)
@@ -393,28 +420,42 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
             buf -= my_k * tile_floats;
 #pragma unroll 1
             for (int e = my_k * 32 + lane; e < tile_floats; e += cut.wk * 32) {
+                const int m = m0 + e / W4_ROWS, n = tile * W4_ROWS + e % W4_ROWS;
+                const bool out = cut.split == 1 && n < a.N;
+                Beside b = {};
+                if (out) b = beside(a, otype, !XG && a.xscales, m, n);
                 float v = 0.f;
                 for (int k = 0; k < cut.wk; ++k) v += buf[k * tile_floats + e];
-                const int m = m0 + e / W4_ROWS, n = tile * W4_ROWS + e % W4_ROWS;
                 if (cut.split > 1) joined[e] = v;
-                else if (n < a.N) put_out(a, xtype, otype, m, n, !XG && a.xscales ? v * a.xscales[m] : v);
+                else if (out) put_out(a, xtype, otype, m, n, v, b);
             }
         }
         if (cut.split == 1) break;
         cl.sync();
         const int all = cut.steps * wt * tile_floats;
 #pragma unroll 1
-        for (int e = rank * W4_THREADS + threadIdx.x; e < all; e += cut.split * W4_THREADS) {
-            const int local = e / tile_floats, i = e - local * tile_floats;
-            const int at = cluster + (batch * cut.steps * wt + local) * cut.clusters;
-            const int m = m0 + i / W4_ROWS, n = at * W4_ROWS + i % W4_ROWS;
-            if (at >= tiles || n >= a.N) continue;
-            float v = 0.f, u[8];
+        for (int e = rank * W4_THREADS + threadIdx.x; e < all; e += 2 * cut.split * W4_THREADS) {
+            int m[2], n[2];
+            float u[2][8];
+            Beside b[2];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) u[k] = k < cut.split ? *cl.map_shared_rank(part + e, k) : 0.f;  // all on their way at once
+            for (int i = 0; i < 2; ++i) {  // two outputs' loads, remote and global, before the first sum
+                const int f = e + i * cut.split * W4_THREADS, local = f / tile_floats, r = f - local * tile_floats;
+                const int at = cluster + (batch * cut.steps * wt + local) * cut.clusters;
+                m[i] = m0 + r / W4_ROWS;
+                n[i] = at * W4_ROWS + r % W4_ROWS;
+                if (f >= all || at >= tiles || n[i] >= a.N) n[i] = -1;
+                if (n[i] >= 0) b[i] = beside(a, otype, !XG && a.xscales, m[i], n[i]);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v += u[k];
-            put_out(a, xtype, otype, m, n, !XG && a.xscales ? v * a.xscales[m] : v);
+                for (int k = 0; k < 8; ++k) u[i][k] = n[i] >= 0 && k < cut.split ? *cl.map_shared_rank(part + f, k) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float v = 0.f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v += u[i][k];
+                if (n[i] >= 0) put_out(a, xtype, otype, m[i], n[i], v, b[i]);
+            }
         }
         cl.sync();  // no block's sums go while another reads them
     }
