@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
             }
 #pragma unroll
             for (int o = 1; o < SUB / 8; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
-            // 2^(14 - exponent of the largest value), in two factors that f32 holds; back is its inverse times 2^24
+            // 2^(14 - exponent of the largest value), in two factors that f32 holds; back is its inverse
             const int up = 14 - max((int)(top >> 23) - 127, -126);
             const float f0 = __uint_as_float((uint32_t)(up / 2 + 127) << 23), f1 = __uint_as_float((uint32_t)(up - up / 2 + 127) << 23);
             back = __uint_as_float((uint32_t)(127 - up / 2) << 23) * __uint_as_float((uint32_t)(127 - up + up / 2) << 23);
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
                 at[0] = at[2] = sum * (-8.f * 0x1p-24f);
                 if constexpr (XG) {
                     if (xtype != TCB_BF16) back = k0 + k < a.K ? __ldg(a.xscales + (int64_t)(m0 + m) * ((a.K + a.xgroup - 1) / a.xgroup) + (k0 + k) / a.xgroup) : 0.f;
-                    at[4] = back * 0x1p24f;
+                    at[4] = back * 0x1p12f;  // the other half of 2^24 at the tile's end, so that neither leaves f32's range
                 }
             }
         }
@@ -386,15 +386,17 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
                     if ((j + 1) * 32 % SUB == 0) {
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            float s0 = su[sub], s1 = su[sub], s2 = sv[sub], s3 = sv[sub];
+                            float v[4];
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) v[c] = fmaf(Y[n][c], 0.0625f, X[n][c]);
                             if constexpr (XG) {
                                 const float2 xf = lds_f32x2(so + (sub * GROUP + 4 * n * PAIR + 4) * 4);
-                                s0 *= xf.x, s1 *= xf.y, s2 *= xf.x, s3 *= xf.y;
+                                v[0] *= xf.x, v[1] *= xf.y, v[2] *= xf.x, v[3] *= xf.y;
                             }
-                            acc[n][0] = fmaf(fmaf(Y[n][0], 0.0625f, X[n][0]), s0, acc[n][0]);
-                            acc[n][1] = fmaf(fmaf(Y[n][1], 0.0625f, X[n][1]), s1, acc[n][1]);
-                            acc[n][2] = fmaf(fmaf(Y[n][2], 0.0625f, X[n][2]), s2, acc[n][2]);
-                            acc[n][3] = fmaf(fmaf(Y[n][3], 0.0625f, X[n][3]), s3, acc[n][3]);
+                            acc[n][0] = fmaf(v[0], su[sub], acc[n][0]);
+                            acc[n][1] = fmaf(v[1], su[sub], acc[n][1]);
+                            acc[n][2] = fmaf(v[2], sv[sub], acc[n][2]);
+                            acc[n][3] = fmaf(v[3], sv[sub], acc[n][3]);
                         }
                     }
                 }
@@ -412,7 +414,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {  // weight row g + 8 (c / 2), token row 8 n + 2 t + c % 2
                     const int m = 8 * n + 2 * t + c % 2;
-                    if (m < rows) buf[m * W4_ROWS + g + c / 2 * 8] = XG ? acc[n][c] : acc[n][c] * 0x1p24f;
+                    if (m < rows) buf[m * W4_ROWS + g + c / 2 * 8] = acc[n][c] * (XG ? 0x1p12f : 0x1p24f);
                 }
             if (cut.wk > 1) asm volatile("bar.sync %0, %1;" ::"r"(my_t + 1), "r"(cut.wk * 32) : "memory");
             else __syncwarp();

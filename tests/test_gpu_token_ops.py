@@ -155,6 +155,66 @@ def test_rmsnorm_codes(lib, M, D, ytype, group):
     rms_case(lib, M, D, 8, tb.F32, ytype, group, True, gamma=False)
 
 
+@pytest.mark.parametrize("D", [8, 15, 16, 17, 57, 64, 65, 249, 250, 256, 257, 505, 512, 513, 761, 768, 1017, 1018, 1024, 1025, 1530,
+                               1536, 1537, 2041, 2048, 2049, 2560, 2561, 2800, 4089, 4097, 8186, 8193, 16377, 16378])
+@pytest.mark.parametrize("pad", [0, 1, 8])
+def test_rmsnorm_team_edges(lib, D, pad):
+    """Widths around the ends of every team, in rows that start on and off the boundaries."""
+    rms_case(lib, 5, D, pad, tb.BF16, tb.E4M3, 64, True, seed=pad)
+    rms_case(lib, 5, D, pad, tb.F32, tb.F32, 0, True, seed=pad)
+    rms_case(lib, 5, D, pad, tb.F16, tb.I8, 0, False, seed=pad)
+
+
+@pytest.mark.parametrize("D,ld", [(640, 640), (1337, 1341), (100, 103), (2560, 2560)])
+@pytest.mark.parametrize("shift", [(1, 1, 1, 1), (3, 3, 3, 3), (1, 0, 0, 0), (0, 2, 5, 0), (0, 0, 0, 1)])
+@pytest.mark.parametrize("ytype", [tb.BF16, tb.I8])
+def test_rmsnorm_shifted_pointers(lib, D, ld, shift, ytype):
+    """x, res, sum and y that start any number of elements behind a boundary, alike or not."""
+    g, M, n = _gen(11), 21, 21 * ld + 8
+    bufs = [_randn(g, n).to(torch.bfloat16) for _ in range(3)] + [torch.zeros(n, device="cuda", dtype=TYPE[ytype])]
+    x, r, sm, y = (b[k:k + M * ld].view(M, ld) for b, k in zip(bufs, shift))
+    w = 1 + 0.1 * _randn(g, D + 1)[1:]
+    group = 32 if ytype == tb.I8 else 0
+    sc = torch.zeros(M, -(-D // group), device="cuda") if group else None
+    h, v = rms_ref(x[:, :D], r[:, :D], w, 1e-6)
+    edges = [b.clone() for b in bufs]
+    assert lib.tcb_op_rmsnorm(_p(x), ld, _p(r), ld, _p(sm), ld, _p(w), 1e-6, tb.BF16, _p(y), ld, ytype, _p(sc), group, M, D,
+                              _stream()) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(sm[:, :D], h)
+    check_rms(h, v, y[:, :D], ytype, group, sc)
+    for b, old, k, written in zip(bufs, edges, shift, (0, 0, 1, 1)):
+        if written:
+            b[k:k + M * ld].view(M, ld)[:, :D] = old[k:k + M * ld].view(M, ld)[:, :D]
+        assert torch.equal(b, old)
+
+
+@pytest.mark.parametrize("D,dtype", [(641, tb.BF16), (99, tb.F32), (3001, tb.F16)])
+def test_rmsnorm_in_place_off_boundaries(lib, D, dtype):
+    """All in place, on rows next to one another: a row's ends share 16 bytes with its neighbours' rows."""
+    g = _gen(12)
+    x, r = _randn(g, 300, D).to(TYPE[dtype]), _randn(g, 300, D).to(TYPE[dtype])
+    h, v = rms_ref(x, r, None, 1e-6)
+    assert lib.tcb_op_rmsnorm(_p(x), D, _p(r), D, _p(r), D, None, 1e-6, dtype, _p(x), D, dtype, None, 0, 300, D, _stream()) == 0
+    assert torch.equal(r, h)
+    check_rms(h, v, x, dtype, 0, None)
+
+
+def test_rmsnorm_without_eps(lib):
+    """eps 0: rows far below 1 are normalised all the same; a row of zeros has no norm."""
+    g = _gen(13)
+    x = _randn(g, 4, 640)
+    x[0] *= 1e-30
+    x[1] *= 1e-37
+    x[2] = 0
+    for dtype in (tb.BF16, tb.F32):
+        xt = x.to(TYPE[dtype])
+        for ytype, group in ((dtype, 0), (tb.I8, 0), (tb.E4M3, 128)):
+            y, _, sc = run_rms(lib, xt, None, None, 640, dtype, ytype, group, eps=0.0)
+            h, v = rms_ref(xt, None, None, 0.0)
+            check_rms(h, v, y, ytype, group, sc)
+
+
 def test_rmsnorm_long(lib):
     """More rows than any grid holds at once."""
     rms_case(lib, 70001, 640, 0, tb.BF16, tb.E4M3, 128, True)
@@ -316,6 +376,26 @@ def test_rope_turns_back_and_gradient(lib):
     assert abs((diff * w.double()).sum().item() - (grad * d.double()).sum().item()) <= n ** 0.5 * scale * 20 * U / eps
 
 
+@pytest.mark.parametrize("shift", [0, 1, 4])
+@pytest.mark.parametrize("dtype", [tb.BF16, tb.F32])
+@pytest.mark.parametrize("inter", [False, True])
+def test_rope_shifted_pointers(lib, shift, dtype, inter):
+    """x and out some elements behind a boundary; rotated parts that are and are not whole vectors of either layout."""
+    g, M, H, hd = _gen(14), 11, 3, 64
+    for rot in (8, 16, 24, 40, 64):
+        buf = _randn(g, M * H * hd + 8).to(TYPE[dtype])
+        out = torch.zeros_like(buf)
+        x = buf[shift:shift + M * H * hd].view(M, H, hd)
+        pos = torch.arange(M, device="cuda", dtype=torch.float32)
+        freq = torch.from_numpy(tb.rope_freqs(rot)[0]).cuda()
+        want, mag = rope_ref(x.double(), pos, freq, 1.0, rot, inter, False)
+        assert lib.tcb_op_rope(buf[shift:].data_ptr(), H * hd, hd, dtype, _p(pos), 1, tb.F32, _p(freq), 1.0, rot, int(inter), 0,
+                               out[shift:].data_ptr(), H * hd, hd, M, H, hd, _stream()) == 0
+        within(out[shift:shift + M * H * hd].view(M, H, hd), want.to(TYPE[dtype]),
+               mag * 10 * U + want.abs() * 2 * HALF[dtype] + TINY[dtype])
+        assert not out[:shift].any() and not out[shift + M * H * hd:].any()
+
+
 def test_rope_far_pitch(lib):
     ld = 1_300_000_008
     buf = torch.empty(2 * ld + 64, dtype=torch.bfloat16, device="cuda")
@@ -404,6 +484,84 @@ def test_gemv_w4_epilogues(lib):
 def test_gemv_w4_largest(lib):
     w4_case(lib, 3, 16384, 8192, 128, tb.BF16, tb.BF16)
     w4_case(lib, 32, 4096, 16384, 64, tb.F16, tb.F16)
+
+
+@pytest.mark.parametrize("M,N,K,xtype", [(1, 40, 65536, tb.BF16), (9, 17, 65500, tb.F16), (3, 33, 40000, tb.E4M3),
+                                         (33, 20, 16384, tb.BF16), (32, 4096, 8192, tb.BF16), (29, 700, 10001, tb.F16),
+                                         (17, 8191, 5001, tb.I8), (300, 70, 700, tb.BF16), (1, 60000, 128, tb.BF16),
+                                         (5, 2000, 7000, tb.F16), (1, 256, 16384, tb.BF16)])
+def test_gemv_w4_cuts(lib, M, N, K, xtype):
+    """Sizes whose token rows or weight rows make the launch split K over clusters, slice a tile's records over warps, join in
+    several batches, or cut the token rows."""
+    for group in (32, 128):
+        w4_case(lib, M, N, K, group, xtype, tb.F32, xgroup=64 if xtype == tb.E4M3 else 0, res=True, pad=1)
+        w4_case(lib, M, N, K, group, xtype, tb.BF16, relu=True)
+
+
+@pytest.mark.parametrize("shift", [1, 2, 4, 8])
+@pytest.mark.parametrize("xtype", [tb.BF16, tb.I8])
+def test_gemv_w4_shifted_x(lib, shift, xtype):
+    """x some elements behind a boundary, with aligned and unaligned pitches."""
+    g = _gen(15)
+    codes = torch.randint(-8, 8, (50, 300), generator=torch.Generator().manual_seed(3), dtype=torch.int8)
+    w = torch.from_numpy(tb.w4_pack(codes.numpy(), 64, np.ones((50, 5), np.float32))).cuda()
+    for ld in (304, 301):
+        buf = (20 * _randn(g, 6 * ld + 16)).round().to(TYPE[xtype])
+        x = buf[shift:shift + 6 * ld].view(6, ld)[:, :300]
+        xs = torch.full((6, 1), 0.5, device="cuda") if xtype == tb.I8 else None
+        y = torch.zeros(6, 50, device="cuda")
+        assert lib.tcb_op_gemv_w4(buf[shift:].data_ptr(), ld, xtype, _p(xs), 0, _p(w), 64, None, 0, None, 0, _p(y), 50, tb.F32,
+                                  6, 50, 300, _stream()) == 0
+        # whole numbers below 2^24 throughout: exact
+        assert torch.equal(y.double(), x.double() @ codes.cuda().double().t() * (0.5 if xtype == tb.I8 else 1))
+
+
+def test_gemv_w4_far_values(lib):
+    """bf16 token rows of any size: each group is scaled by its largest value, which costs what is 2^-31 of it and smaller at
+    most 2^-39 of it; the tolerance adds that times the weights' magnitudes. Sums are held times 2^-12 while subnormal steps
+    are 2^-149: four groups' roundings are 4 x 2^-150 x 2^12 < 2^-135."""
+    g = _gen(16)
+    K, N = 512, 64
+    codes = torch.randint(-8, 8, (N, K), device="cuda", generator=g, dtype=torch.int8)
+    w = torch.from_numpy(tb.w4_pack(codes.cpu().numpy(), 128, np.full((N, 4), 0.125, np.float32))).cuda()
+    x = _randn(g, 8, K)
+    x[0] *= 1e30
+    x[1] *= 1e-30
+    x[2] *= torch.exp(20 * _randn(g, K))
+    x[3] = 0
+    x[4, 128:256] = 0
+    x[5] = 3e38 * torch.sign(x[5]) * (torch.arange(K, device="cuda") == 77)
+    x[6] = 1e-40
+    x[7] *= torch.where(torch.arange(K, device="cuda") % 2 == 0, 1e18, 1e-18)
+    x = x.to(torch.bfloat16)
+    y = torch.zeros(8, N, device="cuda")
+    assert lib.tcb_op_gemv_w4(_p(x), K, tb.BF16, None, 0, _p(w), 128, None, 0, None, 0, _p(y), N, tb.F32, 8, N, K, _stream()) == 0
+    wd = codes.double() * 0.125
+    want, mag = x.double() @ wd.t(), x.double().abs() @ wd.abs().t()
+    tops = x.double().abs().view(8, 4, 128).amax(2).repeat_interleave(128, 1)
+    within(y, want.to(torch.float32), mag * (K + K / 16 + 16) * 2 * U + (tops * 2.0 ** -39) @ wd.abs().t() + 2.0 ** -135)
+
+
+def test_gemv_w4_infinite_results(lib):
+    """An infinity times codes of one sign is that infinity, of both signs NaN, whatever slice or group it is in."""
+    K, N = 2048, 20
+    codes = np.ones((N, K), np.int8)
+    codes[1] = -3
+    codes[2, ::2] = -2
+    codes[3, 5] = 0
+    for at in (5, 1999):
+        w = torch.from_numpy(tb.w4_pack(codes, 128, np.ones((N, 16), np.float32))).cuda()
+        x = torch.ones(3, K, device="cuda")
+        x[0, at] = float("inf")
+        x[1, at] = float("-inf")
+        x[2, at - 1] = x[2, at] = float("inf")
+        for xtype in (tb.BF16, tb.F16):
+            xt = x.to(TYPE[xtype])
+            y = torch.zeros(3, N, device="cuda")
+            assert lib.tcb_op_gemv_w4(_p(xt), K, xtype, None, 0, _p(w), 128, None, 0, None, 0, _p(y), N, tb.F32, 3, N, K,
+                                      _stream()) == 0
+            want = xt.double() @ torch.from_numpy(codes).cuda().double().t()
+            assert torch.equal(torch.nan_to_num(y.double(), 7, 8, 9), torch.nan_to_num(want, 7, 8, 9))
 
 
 def test_gemv_w4_nan_and_inf_stay_in_their_row(lib):
@@ -512,6 +670,35 @@ def test_block_front_captured_and_replayed(lib):
     torch.cuda.synchronize()
     a.check()
     b.check()
+
+
+def test_two_streams_at_once(lib):
+    """The same operators on two streams that overlap, on sizes that split K over clusters."""
+    g = _gen(17)
+    jobs, M, N, K = [], 17, 2000, 10000
+    for _ in range(2):
+        codes = torch.randint(-8, 8, (N, K), device="cuda", generator=g, dtype=torch.int8)
+        w = torch.from_numpy(tb.w4_pack(codes.cpu().numpy(), 128, np.full((N, -(-K // 128)), 0.125, np.float32))).cuda()
+        jobs.append((torch.cuda.Stream(), w, _randn(g, M, K).to(torch.float16), torch.zeros(M, N, device="cuda")))
+    torch.cuda.synchronize()
+
+    def call(st, w, x, y):
+        assert lib.tcb_op_gemv_w4(_p(x), K, tb.F16, None, 0, _p(w), 128, None, 0, None, 0, _p(y), N, tb.F32, M, N, K,
+                                  st.cuda_stream) == 0
+
+    for j in jobs:
+        call(*j)
+    torch.cuda.synchronize()
+    alone = [j[3].clone() for j in jobs]
+    for j in jobs:
+        j[3].zero_()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for j in jobs:
+            call(*j)
+    torch.cuda.synchronize()
+    for j, want in zip(jobs, alone):
+        assert torch.equal(j[3], want)
 
 
 def test_repeated_calls_give_the_same_bits(lib):
