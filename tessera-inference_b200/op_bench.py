@@ -5,6 +5,9 @@ operator entry points (include/tessera_b200_ops.h), with CUDA events.
   python tessera-inference_b200/op_bench.py layernorm --M 131072
   python tessera-inference_b200/op_bench.py gemm --M 524288 --N 2560 --K 640 --mode relu --seconds 3 [--torch]
   python tessera-inference_b200/op_bench.py encode --rows 64 --reps 2      # a profiling driver
+  python tessera-inference_b200/op_bench.py rmsnorm --M 524288 --D 640 --out e4m3 --group 128
+  python tessera-inference_b200/op_bench.py rope --M 524288 --heads 8 --hd 160
+  python tessera-inference_b200/op_bench.py gemv --M 1 --N 16384 --K 8192 --group 128
 
 Prints one JSON line: microseconds per launch, the algorithmic bytes of the
 launch and the bandwidth they give. Attention bytes per token are the Q, K and
@@ -24,6 +27,11 @@ the clock settles under the power cap, and reports TFLOP/s with the median
 SM clock sampled by nvidia-smi over the timed loop (and TFLOP/s per GHz).
 --torch times torch.matmul (cuBLAS, bf16, no epilogue) on the same shape the
 same way, as a comparison point; it is not part of the back end.
+
+`rmsnorm` (bf16 rows with a residual), `rope` (bf16 heads, positions = day of
+year) and `gemv` (4-bit weights, bf16 rows) time the token-stream operators. Their
+launches go over --sets sets of buffers in turn inside a CUDA graph, so host time
+is not in the figure and, with enough sets, nothing is found in L2.
 
 `encode` runs the whole device path (tc_encode_tile_device) --reps times on
 a seeded tile of --rows rows with config 1's width, series lengths and value
@@ -108,9 +116,69 @@ def time_for(fn, seconds: float) -> tuple[float, int, float | None]:
     return us, reps, clk.median()
 
 
+def time_graph(fns, reps: int) -> float:
+    """Microseconds per launch over `reps` rounds of the launches `fns`, replayed as one CUDA graph."""
+    for f in fns:
+        f(torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for f in fns:
+            f(torch.cuda.current_stream().cuda_stream)
+    return time_launches(graph.replay, reps) / len(fns)
+
+
+def token_op(lib, a, g):
+    """(operator, launches, algorithmic bytes of one, sizes) of the token-stream operator that `a` names."""
+    def randn(*n):
+        return torch.randn(*n, device="cuda", generator=g)
+
+    def ok(rc):
+        if rc != 0:
+            raise RuntimeError(f"{a.op} failed")
+
+    fns, M, D, N, K = [], a.M, a.D, a.N, a.K
+    if a.op == "rmsnorm":
+        ytype = {"bf16": tb.BF16, "i8": tb.I8, "e4m3": tb.E4M3}[a.out]
+        group = a.group if a.out != "bf16" else 0
+        ng = -(-D // group) if group else 1
+        gam = 1 + 0.1 * randn(D)
+        for _ in range(a.sets):
+            x, r = randn(M, D).to(torch.bfloat16), randn(M, D).to(torch.bfloat16)
+            h, y = torch.empty_like(x), torch.empty(M, D * (2 if a.out == "bf16" else 1), device="cuda", dtype=torch.uint8)
+            sc = torch.empty(M, ng, device="cuda")
+            fns.append(lambda st, x=x, r=r, h=h, y=y, sc=sc: ok(lib.tcb_op_rmsnorm(
+                x.data_ptr(), D, r.data_ptr(), D, h.data_ptr(), D, gam.data_ptr(), 1e-6, tb.BF16, y.data_ptr(), D, ytype,
+                sc.data_ptr() if a.out != "bf16" else None, group, M, D, st)))
+        nbytes = M * D * (8 if a.out == "bf16" else 7) + (4 * M * ng if a.out != "bf16" else 0)
+        return fns, nbytes, {"M": M, "D": D, "out": a.out, "group": group}
+    if a.op == "rope":
+        width = a.heads * a.hd
+        freq = torch.from_numpy(tb.rope_freqs(a.rot or a.hd)[0]).cuda()
+        for _ in range(a.sets):
+            x = randn(M, width).to(torch.bfloat16)
+            y, pos = torch.empty_like(x), torch.randint(1, 367, (M,), device="cuda", generator=g).float()
+            fns.append(lambda st, x=x, y=y, pos=pos: ok(lib.tcb_op_rope(
+                x.data_ptr(), width, a.hd, tb.BF16, pos.data_ptr(), 1, tb.F32, freq.data_ptr(), 1.0, a.rot or a.hd,
+                int(a.interleaved), 0, y.data_ptr(), width, a.hd, M, a.heads, a.hd, st)))
+        return fns, 4 * M * width, {"M": M, "heads": a.heads, "hd": a.hd, "rot": a.rot or a.hd, "interleaved": a.interleaved}
+    group = a.group or 128
+    nb = lib.tcb_w4_bytes(N, K, group)
+    if nb < 0:
+        raise RuntimeError("bad sizes")
+    for _ in range(a.sets):
+        # any bytes are codes; scales of 2^-8 (bf16 0x3b80) behind each record's 1,024 bytes
+        w = torch.randint(0, 256, (nb,), device="cuda", generator=g, dtype=torch.uint8)
+        w.view(-1, 1024 + 4096 // group)[:, 1024:].view(torch.int16).fill_(0x3b80)
+        x, y = randn(M, K).to(torch.bfloat16), torch.empty(M, N, device="cuda", dtype=torch.bfloat16)
+        fns.append(lambda st, w=w, x=x, y=y: ok(lib.tcb_op_gemv_w4(
+            x.data_ptr(), K, tb.BF16, None, 0, w.data_ptr(), group, None, 0, None, 0, y.data_ptr(), N, tb.BF16, M, N, K, st)))
+    return fns, N * K // 2 + 2 * N * -(-K // group) + 2 * M * (N + K), {"M": M, "N": N, "K": K, "group": group}
+
+
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
-    ap.add_argument("op", choices=["attention", "layernorm", "gemm", "encode"])
+    ap.add_argument("op", choices=["attention", "layernorm", "gemm", "encode", "rmsnorm", "rope", "gemv"])
     ap.add_argument("--rows", type=int, default=64, help="tile rows (encode)")
     ap.add_argument("--N", type=int, default=2560)
     ap.add_argument("--K", type=int, default=640)
@@ -120,7 +188,15 @@ def main(argv=None) -> int:
     ap.add_argument("--torch", action="store_true", help="also time torch.matmul (cuBLAS) on the same shape")
     ap.add_argument("--T", type=int, default=120, help="uniform series length (attention)")
     ap.add_argument("--tokens", type=int, default=131072, help="tokens per attention chunk")
-    ap.add_argument("--M", type=int, default=131072, help="rows (layernorm)")
+    ap.add_argument("--M", type=int, default=131072, help="rows (layernorm, rmsnorm, rope, gemv)")
+    ap.add_argument("--D", type=int, default=640, help="columns (rmsnorm)")
+    ap.add_argument("--out", choices=["bf16", "i8", "e4m3"], default="e4m3", help="output (rmsnorm)")
+    ap.add_argument("--group", type=int, default=0, help="columns per scale (rmsnorm: 0 = the row; gemv: 0 = 128)")
+    ap.add_argument("--heads", type=int, default=8)
+    ap.add_argument("--hd", type=int, default=160)
+    ap.add_argument("--rot", type=int, default=0, help="turned columns of a head (rope: 0 = all)")
+    ap.add_argument("--interleaved", action="store_true", help="pairs (2i, 2i + 1) (rope)")
+    ap.add_argument("--sets", type=int, default=3, help="sets of buffers (rmsnorm, rope, gemv)")
     ap.add_argument("--reps", type=int, default=10)
     a = ap.parse_args(argv)
     lib = tb.load_library()
@@ -139,6 +215,10 @@ def main(argv=None) -> int:
         us = time_launches(run, a.reps)
         nbytes = M * 5120
         rec = {"op": "attention", "tokens": M, "pixels": npix, "T": a.T}
+    elif a.op in ("rmsnorm", "rope", "gemv"):
+        fns, nbytes, rec = token_op(lib, a, g)
+        us = time_graph(fns, a.reps)
+        rec = {"op": a.op, **rec}
     elif a.op == "encode":
         import tempfile as tf
         import synth
