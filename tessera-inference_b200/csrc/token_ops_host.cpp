@@ -40,18 +40,20 @@ void rope_freqs(int rot, double base, int scaling, double factor, double span, d
 }
 
 int64_t w4_bytes(int N, int K, int group) {
-    if (N < 1 || K < 1 || K > 65536 || (group != 32 && group != 64 && group != 128)) return -1;
+    if (N < 1 || N > 1 << 24 || K < 1 || K > 65536 || (group != 32 && group != 64 && group != 128)) return -1;
     const int64_t tiles = ((int64_t)N + W4_ROWS - 1) / W4_ROWS, recs = (K + W4_COLS - 1) / W4_COLS;
     return tiles * recs * w4_record_bytes(group);
 }
 
 void w4_pack_codes(const int8_t *codes, const float *scales, int N, int K, int group, void *packed) {
     const int64_t bytes = w4_bytes(N, K, group);
-    need(bytes > 0, "N < 1, K is not in 1..65536 or group is not 32, 64 or 128");
+    need(bytes > 0, "N is not in 1..2^24, K not in 1..65536 or group not 32, 64 or 128");
     need(codes && scales && packed, "codes, scales or packed is NULL");
     const int recs = (K + W4_COLS - 1) / W4_COLS, rec = w4_record_bytes(group), ng = (K + group - 1) / group;
     for (int64_t i = 0; i < (int64_t)N * K; ++i)
         if (codes[i] < -8 || codes[i] > 7) throw std::runtime_error("a code is not in -8..7");
+    for (int64_t i = 0; i < (int64_t)N * ng; ++i)
+        if (!std::isfinite(__bfloat162float(__float2bfloat16_rn(scales[i])))) throw std::runtime_error("a scale is not finite");
     uint8_t *out = static_cast<uint8_t *>(packed);
     std::memset(out, 0, (size_t)bytes);
     for (int64_t b = 0; b < bytes; b += rec) std::memset(out + b, 0x88, W4_CODE_BYTES);  // q = 0
@@ -73,7 +75,7 @@ void w4_pack_codes(const int8_t *codes, const float *scales, int N, int K, int g
 }
 
 void w4_pack(const float *w, int N, int K, int group, void *packed) {
-    need(w4_bytes(N, K, group) > 0, "N < 1, K is not in 1..65536 or group is not 32, 64 or 128");
+    need(w4_bytes(N, K, group) > 0, "N is not in 1..2^24, K not in 1..65536 or group not 32, 64 or 128");
     need(w && packed, "w or packed is NULL");
     const int ng = (K + group - 1) / group;
     std::vector<int8_t> codes((size_t)N * K);

@@ -672,6 +672,29 @@ def test_block_front_captured_and_replayed(lib):
     b.check()
 
 
+def test_captured_first_and_replayed(lib):
+    """A size that splits K over clusters, whose kernel's first call on the device is the captured one, replayed on other
+    inputs, and a second graph of the same sizes replayed between."""
+    M, N, K, group = 25, 400, 9000, 64
+    g, jobs = _gen(18), []
+    for _ in range(2):
+        codes = torch.randint(-8, 8, (N, K), device="cuda", generator=g, dtype=torch.int8)
+        w = torch.from_numpy(tb.w4_pack(codes.cpu().numpy(), group, np.full((N, -(-K // group)), 0.125, np.float32))).cuda()
+        x, y = torch.zeros(M, K, device="cuda", dtype=torch.float16), torch.zeros(M, N, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            assert lib.tcb_op_gemv_w4(_p(x), K, tb.F16, None, 0, _p(w), group, None, 0, None, 0, _p(y), N, tb.F32, M, N, K,
+                                      _stream()) == 0
+        jobs.append((graph, codes.double() * 0.125, x, y))
+    for _ in range(3):
+        for graph, wd, x, y in jobs:
+            x.copy_(_randn(g, M, K))
+            graph.replay()
+        for graph, wd, x, y in jobs:
+            want, mag = x.double() @ wd.t(), x.double().abs() @ wd.abs().t()
+            within(y, want, mag * (K + K / 16 + 16) * 2 * U + want.abs() * U)
+
+
 def test_two_streams_at_once(lib):
     """The same operators on two streams that overlap, on sizes that split K over clusters."""
     g = _gen(17)

@@ -41,7 +41,11 @@ def _w4(lib, **kw):
     (dict(group=-32), "group is not"), (dict(ytype=tb.BF16, scales=None, group=32), "group without"),
     (dict(ytype=tb.BF16), "scales without"), (dict(scales=None), "scales is NULL"), (dict(ldx=63), "pitch"),
     (dict(ldr=63), "pitch"), (dict(lds=63), "pitch"), (dict(ldy=63), "pitch"), (dict(res=None), "sum without res"),
-    (dict(x=None), "NULL"), (dict(y=None), "NULL"),
+    (dict(x=None), "NULL"), (dict(y=None), "NULL"), (dict(x=P + 1), "aligned"), (dict(res=P + 1), "aligned"),
+    (dict(sum=P + 1), "aligned"), (dict(g=P + 2), "aligned"), (dict(scales=P + 2), "aligned"),
+    (dict(dtype=tb.F32, x=P + 2), "aligned"), (dict(ytype=tb.BF16, scales=None, y=P + 1), "aligned"),
+    (dict(lds=72, y=2 * P), "another pitch"), (dict(ytype=tb.BF16, scales=None, y=3 * P, x=3 * P, ldy=80), "another pitch"),
+    (dict(), "8-bit output over"), (dict(ytype=tb.BF16, scales=None, y=4 * P, res=4 * P, sum=5 * P), "y is res"),
 ])
 def test_rmsnorm_refusals(kw, says, capfd):
     assert _rms(tb.load_library(), **kw) == -1
@@ -56,7 +60,9 @@ def test_rmsnorm_refusals(kw, says, capfd):
     (dict(hsx=31), "head stride"), (dict(hso=31), "head stride"), (dict(pos_stride=-1), "pos_stride"),
     (dict(ldx=-1), "pitch"), (dict(ldo=-128), "pitch"), (dict(ldo=127), "overlap"), (dict(ldo=0), "overlap"),
     (dict(ldo=32, hso=127), "overlap"), (dict(x=None), "NULL"), (dict(pos=None), "NULL"), (dict(freq=None), "NULL"),
-    (dict(out=None), "NULL"), (dict(out=P, ldx=130), "other strides"), (dict(out=P, hsx=33, ldx=132, ldo=132), "other strides"),
+    (dict(out=None), "NULL"), (dict(x=P + 1), "aligned"), (dict(out=2 * P + 1), "aligned"), (dict(pos=P + 2), "aligned"),
+    (dict(pos_type=tb.I64, pos=P + 4), "aligned"), (dict(freq=P + 4), "aligned"),
+    (dict(ldo=2 ** 62, hso=2 ** 62, M=2 ** 40, hd=32), "overlap"), (dict(out=P, ldx=130), "other strides"), (dict(out=P, hsx=33, ldx=132, ldo=132), "other strides"),
 ])
 def test_rope_refusals(kw, says, capfd):
     assert _rope(tb.load_library(), **kw) == -1
@@ -66,12 +72,14 @@ def test_rope_refusals(kw, says, capfd):
 
 @pytest.mark.parametrize("kw,says", [
     (dict(xtype=tb.F32), "xtype"), (dict(xtype=tb.I32), "xtype"), (dict(otype=tb.E4M3), "otype"), (dict(M=-1), "M is not"), (dict(M=2 ** 18 + 1), "M is not"),
-    (dict(N=0), "N < 1"), (dict(K=0), "K is not"), (dict(K=65537, ldx=65537), "K is not"),
+    (dict(N=0), "N is not"), (dict(K=0), "K not"), (dict(K=65537, ldx=65537), "K not"),
     (dict(group=16), "group"), (dict(group=0), "group"), (dict(xgroup=16), "xgroup"),
     (dict(xtype=tb.BF16, xscales=None, xgroup=32), "xgroup without"), (dict(xtype=tb.BF16), "xscales without"),
     (dict(xscales=None), "xscales is NULL"), (dict(ldx=255), "pitch"), (dict(ldo=47), "pitch"), (dict(ldr=47), "pitch"),
     (dict(x=None), "NULL"), (dict(w=None), "NULL"), (dict(out=None), "NULL"), (dict(w=P + 8), "aligned"),
-    (dict(res=2 * P, ldr=49), "another pitch"),
+    (dict(res=2 * P, ldr=49), "another pitch"), (dict(N=2 ** 24 + 1, ldo=2 ** 25, ldr=2 ** 25), "N is not"),
+    (dict(xtype=tb.BF16, xscales=None, x=P + 1), "aligned"), (dict(xscales=P + 2), "aligned"), (dict(bias=P + 2), "aligned"),
+    (dict(res=P + 1), "aligned"), (dict(out=2 * P + 1), "aligned"), (dict(out=P, res=None), "out is x"),
 ])
 def test_gemv_w4_refusals(kw, says, capfd):
     assert _w4(tb.load_library(), **kw) == -1
@@ -168,7 +176,7 @@ def test_w4_pack_quantises(N, K, group):
 
 def test_w4_pack_refusals(capfd):
     lib = tb.load_library()
-    for bad in ((0, 128, 32), (16, 0, 32), (16, 128, 16), (16, 65537, 32), (-1, 128, 32)):
+    for bad in ((0, 128, 32), (16, 0, 32), (16, 128, 16), (16, 65537, 32), (-1, 128, 32), (2 ** 24 + 1, 128, 32)):
         assert lib.tcb_w4_bytes(*bad) == -1
         assert lib.tcb_w4_pack(P, *bad, P) == -1
         assert lib.tcb_w4_pack_codes(P, P, *bad, P) == -1
@@ -176,6 +184,11 @@ def test_w4_pack_refusals(capfd):
     codes, s = np.array([[0, 8, 0, 0]], np.int8), np.ones((1, 1), np.float32)
     assert lib.tcb_w4_pack_codes(tb._ptr(codes), tb._ptr(s), 1, 4, 32, tb._ptr(out)) == -1
     assert "-8..7" in capfd.readouterr().err
+    codes[0, 1] = 7
+    for v in (np.nan, np.inf, 3.4e38):  # the last one rounds to an infinite bf16
+        s[0, 0] = v
+        assert lib.tcb_w4_pack_codes(tb._ptr(codes), tb._ptr(s), 1, 4, 32, tb._ptr(out)) == -1
+        assert "not finite" in capfd.readouterr().err
     for v, says in ((np.nan, "not finite"), (np.inf, "not finite")):
         w = np.array([[0, v, 0, 0]], np.float32)
         assert lib.tcb_w4_pack(tb._ptr(w), 1, 4, 32, tb._ptr(out)) == -1
