@@ -27,6 +27,7 @@ void launch_rmsnorm(RmsArgs a, int dtype, int ytype, cudaStream_t st) {
     need(!codes || (a.y != a.x && a.y != a.res && a.y != a.sum), "8-bit output over its input");
     need(a.y != a.res || !a.res, "y is res");
     a.inv_d = (float)(1.0 / a.D);
+    a.shift = a.group == 128 ? 7 : a.group == 64 ? 6 : 5;
     // Where the rows start, in elements behind a boundary of 8: the same for every tensor, or one element at a time. Groups of
     // columns on rows of several warps need boundaries.
     const auto start = [](const void *p, int bytes) { return reinterpret_cast<uintptr_t>(p) / bytes % 8; };

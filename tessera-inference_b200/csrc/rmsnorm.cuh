@@ -128,11 +128,14 @@ __device__ __forceinline__ float team_sum(float v, float *red) {
     return v;
 }
 
-// Largest magnitude over `lanes` neighbouring lanes, NaN if any is; of magnitudes, which order like their bits.
+// Largest magnitude over `lanes` (2 to 32) neighbouring lanes, NaN if any is; of magnitudes, which order like their bits.
 __device__ __forceinline__ float lanes_max(float v, int lanes) {
     uint32_t b = __float_as_uint(v);
     if (lanes >= 32) return __uint_as_float(__reduce_max_sync(~0u, b));
-    for (int o = 1; o < lanes; o <<= 1) b = max(b, __shfl_xor_sync(~0u, b, o));
+    b = max(b, __shfl_xor_sync(~0u, b, 1));
+    if (lanes > 2) b = max(b, __shfl_xor_sync(~0u, b, 2));
+    if (lanes > 4) b = max(b, __shfl_xor_sync(~0u, b, 4));
+    if (lanes > 8) b = max(b, __shfl_xor_sync(~0u, b, 8));
     return __uint_as_float(b);
 }
 template <int TEAM>
@@ -361,7 +364,7 @@ __global__ void __launch_bounds__(RmsShape<T, TEAM, NU, MODE>::THREADS, RmsShape
                 put(y, i, u);
             }
         } else {
-            const int ng = a.group ? (a.D + a.group - 1) / a.group : 1;
+            const int ng = a.group ? (a.D + a.group - 1) >> a.shift : 1;
             float *scales = a.scales + r * ng;
             const auto top_of = [](const float (&p)[8]) {
                 float m = 0.f;
@@ -396,7 +399,7 @@ __global__ void __launch_bounds__(RmsShape<T, TEAM, NU, MODE>::THREADS, RmsShape
                     float p[8];
                     weighted(i, p);
                     const Step s = step_of<Y>(lanes_max(top_of(p), lanes), rstd);
-                    if (t % lanes == 0 && col(i, 0) < D) scales[col(i, 0) / a.group] = s.s;
+                    if ((t & (lanes - 1)) == 0 && col(i, 0) < D) scales[col(i, 0) >> a.shift] = s.s;
                     write(i, codes8<Y>(p, s));
                 }
             } else if constexpr (MODE == EDGED) {
@@ -425,7 +428,7 @@ __global__ void __launch_bounds__(RmsShape<T, TEAM, NU, MODE>::THREADS, RmsShape
                     } else if (t == TEAM - 1) next = 0.f;
                     const Step s = step_of<Y>(lanes_max(max_nan(own[i], next), lanes), rstd);
                     const int at = col(i, 0) + o;
-                    if (t % lanes == 0 && at < D) scales[at / a.group] = s.s;
+                    if ((t & (lanes - 1)) == 0 && at < D) scales[at >> a.shift] = s.s;
                     Step f = {__shfl_up_sync(~0u, s.k, 1, TEAM), __shfl_up_sync(~0u, s.s, 1, TEAM)};
                     if (t == 0) f = before;
                     before = {__shfl_sync(~0u, s.k, TEAM - 1, TEAM), __shfl_sync(~0u, s.s, TEAM - 1, TEAM)};
@@ -455,9 +458,9 @@ __global__ void __launch_bounds__(RmsShape<T, TEAM, NU, MODE>::THREADS, RmsShape
                     uint32_t w[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        if (j % min(values, 8) == 0) {
+                        if ((j & (min(values, 8) - 1)) == 0) {
                             s = step_of<Y>(lanes_max(m[j], TEAM), rstd);
-                            if (t == 0 && col(i, j) < D) scales[col(i, j) / a.group] = s.s;
+                            if (t == 0 && col(i, j) < D) scales[col(i, j) >> a.shift] = s.s;
                         }
                         w[j] = codes4<Y>(p[j], 0.f, 0.f, 0.f, s) & 0xff;
                     }
@@ -474,7 +477,7 @@ __global__ void __launch_bounds__(RmsShape<T, TEAM, NU, MODE>::THREADS, RmsShape
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const uint32_t w = __reduce_max_sync(~0u, magnitude(p[j]));
-                        if (t % 32 == 0 && col(i, j) < D) atomicMax(&gtop[col(i, j) / a.group], w);
+                        if (t % 32 == 0 && col(i, j) < D) atomicMax(&gtop[col(i, j) >> a.shift], w);
                     }
                 }
                 __syncthreads();
@@ -486,8 +489,8 @@ __global__ void __launch_bounds__(RmsShape<T, TEAM, NU, MODE>::THREADS, RmsShape
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const int c = min(col(i, j), D - 1);
-                        const Step s = step_of<Y>(__uint_as_float(gtop[c / a.group]), rstd);
-                        if (col(i, j) < D && c % a.group == 0) scales[c / a.group] = s.s;
+                        const Step s = step_of<Y>(__uint_as_float(gtop[c >> a.shift]), rstd);
+                        if (col(i, j) < D && (c & (a.group - 1)) == 0) scales[c >> a.shift] = s.s;
                         w[j] = codes4<Y>(p[j], 0.f, 0.f, 0.f, s) & 0xff;
                     }
                     write(i, make_uint2(w[0] | w[1] << 8 | w[2] << 16 | w[3] << 24, w[4] | w[5] << 8 | w[6] << 16 | w[7] << 24));

@@ -15,8 +15,11 @@ struct RmsArgs {
     int64_t ldx = 0, ldr = 0, lds = 0, ldy = 0, M = 0;
     const float *g = nullptr;
     float *scales = nullptr;
-    float eps = 0.f, inv_d = 0.f;  // inv_d = 1 / D, set by the launcher
-    int D = 0, group = 0;          // group 0 = the whole row
+    float eps = 0.f;
+    int D = 0, group = 0;  // group 0 = the whole row
+    // set by the launcher
+    float inv_d = 0.f;  // 1 / D
+    int shift = 0;      // log2 group
 };
 void launch_rmsnorm(RmsArgs a, int dtype, int ytype, cudaStream_t st);
 
