@@ -19,13 +19,14 @@ constexpr int ROPE_THREADS = 256;
 
 // Blocks per SM, which bound the registers, and the heads whose loads a thread issues together. Many threads with few loads
 // each hide HBM better than the reverse: on 524,288 rows of 8 heads x 160 in bf16, 6 blocks and one head (two vectors) take
-// 440 us, 4 and two heads 501, 2 and four heads 538.
+// 440 us, 4 and two heads 501, 2 and four heads 538. Narrower vectors take more heads.
 template <class T, bool INTER, int V>
 struct RopeShape {
     static constexpr bool ONE = INTER && V > 1;  // a unit is one vector
-    static constexpr bool WIDE = sizeof(T) == 4 && V > 1;
+    static constexpr int BYTES = V * sizeof(T);
+    static constexpr bool WIDE = sizeof(T) == 4 && BYTES == 16;
     static constexpr int BLOCKS = WIDE ? 5 : 6;
-    static constexpr int AHEAD = V == 1 ? 4 : (ONE ? 2 : 1) * (WIDE ? 2 : 1);
+    static constexpr int AHEAD = BYTES == 16 ? (ONE ? 2 : 1) * (WIDE ? 2 : 1) : BYTES == 8 && !ONE ? 2 : 4;
 };
 
 // cos and sin (times mscale) of pos * freq. The angle is reduced to a fraction
@@ -38,29 +39,29 @@ __device__ __forceinline__ float2 turn_of(double pos, double freq, float mscale,
     return make_float2(c * mscale, s * mscale * sign);
 }
 
-// V elements at once: 16 bytes, or a single element.
+// V elements at once, up to 16 bytes.
 template <class T, int V>
 struct Vec {
     T v[V];
 };
+template <int BYTES>
+struct Word {
+    using type = std::conditional_t<BYTES == 16, uint4, std::conditional_t<BYTES == 8, uint2, std::conditional_t<BYTES == 4, uint32_t, uint16_t>>>;
+};
 template <class T, int V>
 __device__ __forceinline__ Vec<T, V> load(const T *p) {
+    using W = typename Word<V * sizeof(T)>::type;
+    const W q = *reinterpret_cast<const W *>(p);
     Vec<T, V> r;
-    if constexpr (V == 1) r.v[0] = *p;
-    else {
-        const uint4 q = *reinterpret_cast<const uint4 *>(p);
-        memcpy(&r, &q, 16);
-    }
+    memcpy(&r, &q, sizeof(W));
     return r;
 }
 template <class T, int V>
 __device__ __forceinline__ void store(T *p, const Vec<T, V> &r) {
-    if constexpr (V == 1) *p = r.v[0];
-    else {
-        uint4 q;
-        memcpy(&q, &r, 16);
-        *reinterpret_cast<uint4 *>(p) = q;
-    }
+    using W = typename Word<V * sizeof(T)>::type;
+    W q;
+    memcpy(&q, &r, sizeof(W));
+    *reinterpret_cast<W *>(p) = q;
 }
 
 // Units of a row: first those that turn, then those that are copied (none when
@@ -131,27 +132,23 @@ void launch(const RopeArgs &a, cudaStream_t st) {
     k_rope<T, P, INTER, V><<<grid, ROPE_THREADS, 0, st>>>(a, units, rows, slice);
 }
 
-template <class T, class P>
+// The widest vectors, of V columns or fewer, that the pairs, the copied columns and every row and head are whole multiples of.
+template <class T, class P, int V>
 void launch_v(const RopeArgs &a, bool inter, cudaStream_t st) {
-    constexpr int V = 16 / sizeof(T);
-    const auto at = [](const void *p, int64_t ld, int64_t hs) {
-        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % V == 0 && hs % V == 0;
-    };
-    // the pairs, the copied columns, and every row and head in whole vectors
-    if (a.rot % (inter ? V : 2 * V) == 0 && (a.hd - a.rot) % V == 0 && at(a.x, a.ldx, a.hsx) && at(a.out, a.ldo, a.hso)) {
-        if (inter) launch<T, P, true, V>(a, st);
-        else launch<T, P, false, V>(a, st);
-    } else {
-        if (inter) launch<T, P, true, 1>(a, st);
-        else launch<T, P, false, 1>(a, st);
+    const auto at = [](const void *p, int64_t ld, int64_t hs) { return on(p, V * sizeof(T)) && ld % V == 0 && hs % V == 0; };
+    if constexpr (V > 1) {
+        if (a.rot % (inter ? V : 2 * V) || (a.hd - a.rot) % V || !at(a.x, a.ldx, a.hsx) || !at(a.out, a.ldo, a.hso))
+            return launch_v<T, P, V / 2>(a, inter, st);
     }
+    if (inter) launch<T, P, true, V>(a, st);
+    else launch<T, P, false, V>(a, st);
 }
 
 template <class T>
 void launch_p(const RopeArgs &a, int pos_type, bool inter, cudaStream_t st) {
-    if (pos_type == TCB_F32) launch_v<T, float>(a, inter, st);
-    else if (pos_type == TCB_I32) launch_v<T, int32_t>(a, inter, st);
-    else launch_v<T, int64_t>(a, inter, st);
+    if (pos_type == TCB_F32) launch_v<T, float, 16 / sizeof(T)>(a, inter, st);
+    else if (pos_type == TCB_I32) launch_v<T, int32_t, 16 / sizeof(T)>(a, inter, st);
+    else launch_v<T, int64_t, 16 / sizeof(T)>(a, inter, st);
 }
 
 }  // namespace
