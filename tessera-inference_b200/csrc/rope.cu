@@ -84,11 +84,15 @@ __global__ void __launch_bounds__(ROPE_THREADS, RopeShape<T, INTER, V>::BLOCKS) 
             const int p = !turns ? a.rot + (u - turning) * V : INTER ? 2 * PAIRS * u : V * u;
             const int second = INTER ? 1 : half;  // from a pair's first element to its second
             float2 t[PAIRS];
-            if (turns) {
+            const auto angles = [&] {
                 const double pos = (double)static_cast<const P *>(a.pos)[r * a.pos_stride];
 #pragma unroll
                 for (int j = 0; j < PAIRS; ++j) t[j] = turn_of(pos, a.freq[u * PAIRS + j], a.mscale, a.sign);
-            }
+            };
+            // Before the loads for the widest unit, whose registers they would take (524,288 x 8 x 160 in bf16: 440 us, 517 with
+            // them behind); while the first heads' loads are on their way for the others (131,072 x 3 x 151: 127 us, was 139).
+            constexpr bool BEHIND = ONE || V * sizeof(T) < 16;
+            if (!BEHIND && turns) angles();
             const T *x = static_cast<const T *>(a.x) + r * a.ldx + h0 * a.hsx + p;
             T *o = static_cast<T *>(a.out) + r * a.ldo + h0 * a.hso + p;
             for (int h = h0; h < h1; h += AHEAD, x += AHEAD * a.hsx, o += AHEAD * a.hso) {
@@ -99,6 +103,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, RopeShape<T, INTER, V>::BLOCKS) 
                         b[k] = load<T, V>(x + k * a.hsx);
                         if (!ONE && turns) c[k] = load<T, V>(x + k * a.hsx + second);
                     }
+                if (BEHIND && h == h0 && turns) angles();
 #pragma unroll
                 for (int k = 0; k < AHEAD; ++k)
                     if (h + k < h1) {
