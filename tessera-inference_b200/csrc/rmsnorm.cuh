@@ -14,7 +14,7 @@
 // three inputs; f32 arithmetic in the definition's order: 62, 44 and 58).
 //
 // Measured, bf16 rows: 524,288 x 640 with the residual to e4m3 with scales of 128
-// columns in 392 us (6.0 TB/s), to bf16 in 390 us (6.9 TB/s); 32,768 x 2,560 to e4m3
+// columns in 343 us (6.9 TB/s), to bf16 in 391 us (6.9 TB/s); 32,768 x 2,560 to e4m3
 // in 50 us (5.0 TB/s); 8,192 x 16,384 with the residual to int8 in 142 us (6.6 TB/s);
 // fp16 rows of 1,337 at a pitch of 1,341 to int8, 10,007 of them, in 34 us (2.8 TB/s,
 // bound by instructions: weights and edges come one by one).
@@ -209,7 +209,7 @@ enum RmsMode { ALIGNED, EDGED, SINGLE };
 template <class T, int TEAM, int NU, RmsMode MODE>
 struct RmsShape {
     static constexpr int THREADS = TEAM <= 32 ? 128 : TEAM;
-    static constexpr int PACKED = NU <= 2 ? 40 : NU == 3 ? 48 : NU == 4 ? 64 : NU == 5 ? 80 : 96;
+    static constexpr int PACKED = NU <= 2 ? 40 : NU == 3 ? (TEAM == 32 ? 48 : 56) : NU == 4 ? 64 : NU == 5 ? 80 : 96;
     static constexpr int REGS = MODE == EDGED ? (24 + 16 * NU) * (sizeof(T) == 4 ? 5 : 4) / 4
                                 : sizeof(T) == 4 && NU > 1 ? PACKED + 16 : PACKED;
     static constexpr int BLOCKS = 65536 / (THREADS * REGS);
@@ -506,8 +506,9 @@ void rms_launch(const RmsArgs &a, cudaStream_t st) {
     k_rmsnorm<T, Y, TEAM, NU, MODE><<<(unsigned)std::min<int64_t>((a.M + rows - 1) / rows, 1 << 30), threads, 0, st>>>(a);
 }
 
-// The smallest team that holds the row (and up to 7 columns in front of it). Loads outside the row are skipped, so a few
-// sizes serve all widths.
+// The team whose registers hold the row (and up to 7 columns in front of it) with the least to spare, as far as a few sizes
+// serve all widths; loads outside the row are skipped. Two rows of 80 units a warp take 343 us on
+// 524,288 x 640 (bf16 to e4m3), a row a warp, with a sixth of it idle, 363; on one row 2.9 and 2.2.
 template <class T, class Y, RmsMode MODE>
 void rms_launch_team(const RmsArgs &a, cudaStream_t st) {
     const int units = (a.D + RMS_UNIT - 1 + (MODE == EDGED ? 7 : 0)) / RMS_UNIT;
@@ -516,6 +517,7 @@ void rms_launch_team(const RmsArgs &a, cudaStream_t st) {
     if (units <= 32) return rms_launch<T, Y, 32, 1, MODE>(a, st);
     if constexpr (MODE != SINGLE) {
         if (units <= 64) return rms_launch<T, Y, 32, 2, MODE>(a, st);
+        if (MODE == ALIGNED && units <= 80 && a.M >= 2048) return rms_launch<T, Y, 16, 5, MODE>(a, st);
         if (units <= 96) return rms_launch<T, Y, 32, 3, MODE>(a, st);
     }
     if (units <= 128) return rms_launch<T, Y, 32, 4, MODE>(a, st);

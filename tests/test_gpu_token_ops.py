@@ -155,7 +155,7 @@ def test_rmsnorm_codes(lib, M, D, ytype, group):
     rms_case(lib, M, D, 8, tb.F32, ytype, group, True, gamma=False)
 
 
-@pytest.mark.parametrize("D", [8, 15, 16, 17, 57, 64, 65, 249, 250, 256, 257, 505, 512, 513, 761, 768, 1017, 1018, 1024, 1025, 1530,
+@pytest.mark.parametrize("D", [8, 15, 16, 17, 57, 64, 65, 249, 250, 256, 257, 505, 512, 513, 520, 640, 648, 761, 768, 1017, 1018, 1024, 1025, 1530,
                                1536, 1537, 2041, 2048, 2049, 2560, 2561, 2800, 4089, 4097, 8186, 8193, 16377, 16378])
 @pytest.mark.parametrize("pad", [0, 1, 8])
 def test_rmsnorm_team_edges(lib, D, pad):
@@ -685,12 +685,12 @@ def test_captured_first_and_replayed(lib):
         with torch.cuda.graph(graph):
             assert lib.tcb_op_gemv_w4(_p(x), K, tb.F16, None, 0, _p(w), group, None, 0, None, 0, _p(y), N, tb.F32, M, N, K,
                                       _stream()) == 0
-        jobs.append((graph, codes.double() * 0.125, x, y))
+        jobs.append((graph, codes.double() * 0.125, x, y, w))  # w: the graph reads it
     for _ in range(3):
-        for graph, wd, x, y in jobs:
+        for graph, _, x, _, _ in jobs:
             x.copy_(_randn(g, M, K))
             graph.replay()
-        for graph, wd, x, y in jobs:
+        for _, wd, x, y, _ in jobs:
             want, mag = x.double() @ wd.t(), x.double().abs() @ wd.abs().t()
             within(y, want, mag * (K + K / 16 + 16) * 2 * U + want.abs() * U)
 
