@@ -6,9 +6,10 @@
 //
 // Measured: 524,288 rows of 8 heads x 160 in bf16, halves paired, 435 us (6.2 TB/s);
 // 131,072 rows of 10 x 128 with 64 turned columns, interleaved, 106 us (6.4 TB/s);
-// 141,877 rows of 5 x 224 in f32 193 us (6.6 TB/s). Rows that no vector fits (50,000
-// of 10 x 75, 50 turned) go element by element: 55 us (2.7 TB/s).
+// 141,877 rows of 5 x 224 in f32 193 us (6.6 TB/s); heads that no vector fits,
+// 131,072 rows of 8 x 151 in bf16 with 90 turned, 125 us (5.1 TB/s).
 #include <algorithm>
+#include <atomic>
 
 #include "token_ops.cuh"
 
@@ -16,6 +17,7 @@ namespace tcb {
 namespace {
 
 constexpr int ROPE_THREADS = 256;
+constexpr int ROPE_SMEM = 96 * 1024, ROPE_SM_SMEM = 227 * 1024;  // of a block that holds rows, and of an SM
 
 // Blocks per SM, which bound the registers, and the heads whose loads a thread issues together. Many threads with few loads
 // each hide HBM better than the reverse: on 524,288 rows of 8 heads x 160 in bf16, 6 blocks and one head (two vectors) take
@@ -137,6 +139,101 @@ void launch(const RopeArgs &a, cudaStream_t st) {
     k_rope<T, P, INTER, V><<<grid, ROPE_THREADS, 0, st>>>(a, units, rows, slice);
 }
 
+// Rows that take vectors of 4 bytes or less, in packed heads: a warp brings a whole row to shared memory in 16-byte copies,
+// the next one while it works, turns the pairs there element by element, and writes the row back in 16-byte stores. x and out
+// rows start equally far behind 16-byte boundaries; a row's first and last bytes go alone where the 16 are not all its own.
+template <class T, class P, bool INTER>
+__global__ void __launch_bounds__(ROPE_THREADS) k_rope_rows(const RopeArgs a, const int bytes) {
+    extern __shared__ __align__(16) uint8_t tiles[];
+    const int lane = threadIdx.x & 31, half = a.rot / 2, pieces = bytes / 16 + 2, pitch = pieces * 16;
+    uint8_t *mine = tiles + (threadIdx.x >> 5) * 2 * pitch;
+    const int64_t stride = (int64_t)gridDim.x * (blockDim.x >> 5);
+    const uint8_t *const first = static_cast<const uint8_t *>(a.x);
+    const uint8_t *const end = first + (a.M - 1) * a.ldx * (int64_t)sizeof(T) + bytes;  // of x's last row
+    const auto fetch = [&](int64_t r, int slot) {
+        if (r < a.M) {
+            const uint8_t *row = first + r * a.ldx * (int64_t)sizeof(T);
+            const int off = (int)(reinterpret_cast<uintptr_t>(row) % 16);
+            uint8_t *to = mine + slot * pitch;
+            for (int q = lane; q < pieces; q += 32) {
+                const uint8_t *p = row - off + q * 16;
+                if (p >= first && p + 16 <= end) {  // may hold bytes between rows too
+                    if (q * 16 - off < bytes) cp_async16(smem_u32(to + q * 16), p);
+                } else {
+                    for (int j = 0; j < 16; j += (int)sizeof(T))
+                        if (p + j >= row && p + j < row + bytes)
+                            *reinterpret_cast<T *>(to + q * 16 + j) = *reinterpret_cast<const T *>(p + j);
+                }
+            }
+        }
+        cp_async_commit();
+    };
+    // with fewer pairs than lanes, the heads are dealt out to several lanes of a pair
+    const int slices = half < 32 ? 32 / half : 1, slice = half < 32 ? lane / half : 0, own = half < 32 ? lane % half : lane;
+    int64_t r = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    int slot = 0;
+    fetch(r, 0);
+    for (; r < a.M; r += stride, slot ^= 1) {
+        fetch(r + stride, slot ^ 1);
+        cp_async_wait<1>();
+        __syncwarp();
+        uint8_t *tile = mine + slot * pitch;
+        const int off = (int)((reinterpret_cast<uintptr_t>(a.x) + r * a.ldx * sizeof(T)) % 16);
+        if (slice < slices) {
+            const double pos = (double)static_cast<const P *>(a.pos)[r * a.pos_stride];
+            for (int i = own; i < half; i += 32) {
+                const float2 t = turn_of(pos, a.freq[i], a.mscale, a.sign);
+                T *p = reinterpret_cast<T *>(tile + off) + (INTER ? 2 * i : i), *q = p + (INTER ? 1 : half);
+#pragma unroll 4
+                for (int h = slice; h < a.heads; h += slices) {
+                    const float v = to_f32(p[h * a.hd]), w = to_f32(q[h * a.hd]);
+                    p[h * a.hd] = from_f32<T>(v * t.x - w * t.y);
+                    q[h * a.hd] = from_f32<T>(v * t.y + w * t.x);
+                }
+            }
+        }
+        __syncwarp();
+        uint8_t *row = static_cast<uint8_t *>(a.out) + r * a.ldo * (int64_t)sizeof(T);
+        for (int q = lane; q < pieces; q += 32) {
+            const int b = q * 16 - off;
+            if (b >= 0 && b + 16 <= bytes) *reinterpret_cast<uint4 *>(row + b) = *reinterpret_cast<const uint4 *>(tile + q * 16);
+            else {
+                for (int j = 0; j < 16; j += (int)sizeof(T))
+                    if (b + j >= 0 && b + j < bytes) *reinterpret_cast<T *>(row + b + j) = *reinterpret_cast<const T *>(tile + q * 16 + j);
+            }
+        }
+        __syncwarp();  // the slot is free
+    }
+}
+
+// Launches k_rope_rows where it fits. Long streams only, since it spreads no heads, and rows that give a warp enough to do:
+// 131,072 rows of 8 x 151 (bf16, 90 turned) take 125 us, 219 without it, of 3 x 151 86 and 127; 500,000 rows of 2 x 15 would
+// take 198, 54 without it.
+template <class T, class P>
+bool launch_rows(const RopeArgs &a, bool inter, cudaStream_t st) {
+    const int64_t bytes = (int64_t)a.heads * a.hd * sizeof(T), pitch = (bytes / 16 + 2) * 16;
+    if (a.M < 2048 || bytes < 512 || (a.heads > 1 && (a.hsx != a.hd || a.hso != a.hd)) || a.ldx * (int64_t)sizeof(T) < bytes) return false;
+    if ((reinterpret_cast<uintptr_t>(a.x) - reinterpret_cast<uintptr_t>(a.out)) % 16 || (a.ldx - a.ldo) * (int64_t)sizeof(T) % 16) return false;
+    int warps = ROPE_THREADS / 32;
+    while (warps > 1 && warps * 2 * pitch > ROPE_SMEM) warps /= 2;
+    if (warps * 2 * pitch > ROPE_SMEM) return false;
+    const auto kernel = inter ? k_rope_rows<T, P, true> : k_rope_rows<T, P, false>;
+    static std::atomic<int> known[64][2];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int sms = known[dev & 63][inter].load(std::memory_order_relaxed);
+    if (!sms) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ROPE_SMEM);
+        need(e == cudaSuccess, cudaGetErrorString(e));
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        known[dev & 63][inter].store(sms, std::memory_order_relaxed);
+    }
+    const int smem = (int)(warps * 2 * pitch);
+    const int64_t blocks = std::min<int64_t>((a.M + warps - 1) / warps, (int64_t)sms * std::min(64 / warps, ROPE_SM_SMEM / (smem + 1024)));
+    kernel<<<(unsigned)blocks, warps * 32, smem, st>>>(a, (int)bytes);
+    return true;
+}
+
 // The widest vectors, of V columns or fewer, that the pairs, the copied columns and every row and head are whole multiples of.
 template <class T, class P, int V>
 void launch_v(const RopeArgs &a, bool inter, cudaStream_t st) {
@@ -144,6 +241,9 @@ void launch_v(const RopeArgs &a, bool inter, cudaStream_t st) {
     if constexpr (V > 1) {
         if (a.rot % (inter ? V : 2 * V) || (a.hd - a.rot) % V || !at(a.x, a.ldx, a.hsx) || !at(a.out, a.ldo, a.hso))
             return launch_v<T, P, V / 2>(a, inter, st);
+    }
+    if constexpr (V * sizeof(T) <= 4) {
+        if (launch_rows<T, P>(a, inter, st)) return;
     }
     if (inter) launch<T, P, true, V>(a, st);
     else launch<T, P, false, V>(a, st);

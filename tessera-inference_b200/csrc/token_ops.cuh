@@ -44,6 +44,16 @@ __device__ __forceinline__ T from_f32(float v) {
     else return v;
 }
 
+// Asynchronous copies of 16 bytes into shared memory; a thread sees its own after the wait.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Largest magnitude of an 8-bit code.
 template <class T>
 __host__ __device__ constexpr float code_top() {

@@ -396,6 +396,37 @@ def test_rope_shifted_pointers(lib, shift, dtype, inter):
         assert not out[:shift].any() and not out[shift + M * H * hd:].any()
 
 
+@pytest.mark.parametrize("dtype", [tb.BF16, tb.F16, tb.F32])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("heads,hd,rot", [(8, 151, 90), (1, 3, 2), (3, 51, 26), (19, 208, 82), (5, 66, 64), (40, 255, 254), (1, 1023, 6),
+                                          (100, 257, 130)])
+def test_rope_long_odd(lib, heads, hd, rot, dtype, inter):
+    """Long streams of heads that no vector fits: packed, with columns behind the heads, in place, and in gaps."""
+    rope_case(lib, 2500, heads, hd, rot, dtype, inter, False, span=366)
+    rope_case(lib, 2049, heads, hd, rot, dtype, inter, True, gap=16 if heads < 50 else 0, pos_type=tb.I64, span=9999)
+    rope_case(lib, 2049, heads, hd, rot, dtype, inter, False, gap=5, in_place=True)
+    if heads < 50:
+        rope_case(lib, 2050, heads, hd, rot, dtype, inter, False, hgap=1)
+
+
+@pytest.mark.parametrize("shift", [0, 1, 3, 7])
+def test_rope_long_odd_shifted(lib, shift):
+    """The same with x and out that start off a boundary, alike and not."""
+    g, M, H, hd, rot = _gen(19), 2100, 3, 37, 22
+    for other in (shift, shift + 8, shift + 2):
+        buf = _randn(g, M * H * hd + 16).to(torch.bfloat16)
+        out = torch.zeros_like(buf)
+        x = buf[shift:shift + M * H * hd].view(M, H, hd)
+        pos = torch.arange(M, device="cuda", dtype=torch.int32)
+        freq = torch.from_numpy(tb.rope_freqs(rot)[0]).cuda()
+        want, mag = rope_ref(x.double(), pos, freq, 1.0, rot, False, False)
+        assert lib.tcb_op_rope(buf[shift:].data_ptr(), H * hd, hd, tb.BF16, _p(pos), 1, tb.I32, _p(freq), 1.0, rot, 0, 0,
+                               out[other:].data_ptr(), H * hd, hd, M, H, hd, _stream()) == 0
+        within(out[other:other + M * H * hd].view(M, H, hd), want.to(torch.bfloat16),
+               mag * 10 * U + want.abs() * 2.0 ** -7 + TINY[tb.BF16])
+        assert not out[:other].any() and not out[other + M * H * hd:].any()
+
+
 def test_rope_far_pitch(lib):
     ld = 1_300_000_008
     buf = torch.empty(2 * ld + 64, dtype=torch.bfloat16, device="cuda")
