@@ -123,6 +123,7 @@ enum {
  * tcb_op_out128. Statistics are f32 and do not overflow for finite h. A NaN
  * makes its whole row NaN; an infinity makes its own v NaN and the row's other
  * v zero. A group with a NaN gets the scale NaN, int8 codes 0, e4m3 codes NaN.
+ * A row's result does not depend on M or on the other rows.
  * sum may be x or res itself, and y of dtype may be x or sum (same pitch);
  * other overlaps are not allowed. */
 int tcb_op_rmsnorm(const void *x, int64_t ldx, const void *res, int64_t ldr, void *sum, int64_t lds, const float *g,

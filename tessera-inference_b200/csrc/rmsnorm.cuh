@@ -507,8 +507,9 @@ void rms_launch(const RmsArgs &a, cudaStream_t st) {
 }
 
 // The team whose registers hold the row (and up to 7 columns in front of it) with the least to spare, as far as a few sizes
-// serve all widths; loads outside the row are skipped. Two rows of 80 units a warp take 343 us on
-// 524,288 x 640 (bf16 to e4m3), a row a warp, with a sixth of it idle, 363; on one row 2.9 and 2.2.
+// serve all widths; loads outside the row are skipped. Two rows of 80 units a warp take 343 us on 524,288 x 640 (bf16 to
+// e4m3), a row a warp, with a sixth of it idle, 363; on a single row 2.9 and 2.2. The number of rows has no say, so that a
+// row's bits are the same in any batch.
 template <class T, class Y, RmsMode MODE>
 void rms_launch_team(const RmsArgs &a, cudaStream_t st) {
     const int units = (a.D + RMS_UNIT - 1 + (MODE == EDGED ? 7 : 0)) / RMS_UNIT;
@@ -517,7 +518,7 @@ void rms_launch_team(const RmsArgs &a, cudaStream_t st) {
     if (units <= 32) return rms_launch<T, Y, 32, 1, MODE>(a, st);
     if constexpr (MODE != SINGLE) {
         if (units <= 64) return rms_launch<T, Y, 32, 2, MODE>(a, st);
-        if (MODE == ALIGNED && units <= 80 && a.M >= 2048) return rms_launch<T, Y, 16, 5, MODE>(a, st);
+        if (MODE == ALIGNED && units <= 80) return rms_launch<T, Y, 16, 5, MODE>(a, st);
         if (units <= 96) return rms_launch<T, Y, 32, 3, MODE>(a, st);
     }
     if (units <= 128) return rms_launch<T, Y, 32, 4, MODE>(a, st);

@@ -200,6 +200,39 @@ def test_rmsnorm_in_place_off_boundaries(lib, D, dtype):
     check_rms(h, v, x, dtype, 0, None)
 
 
+def test_rmsnorm_row_alone(lib):
+    """A row's bits are the same alone and in a long stream."""
+    g = _gen(20)
+    for D, group in ((640, 128), (37, 32), (64, 0), (1337, 0), (2560, 64), (9000, 0)):
+        x = _randn(g, 5000, D).to(torch.bfloat16)
+        y, _, sc = run_rms(lib, x, None, None, D, tb.BF16, tb.E4M3, group)
+        for r in (0, 1, 2499, 4999):
+            start = x[r].data_ptr() // 2 % 8  # where the row starts in the stream
+            one = torch.zeros(1, D + 16, device="cuda", dtype=torch.bfloat16)
+            z = torch.zeros(D + 16, device="cuda", dtype=torch.uint8)
+            s = torch.zeros_like(sc[:1])
+            at = (start - one.data_ptr() // 2) % 8
+            k = (at + one.data_ptr() // 2 - z.data_ptr()) % 8
+            one[0, at:at + D] = x[r]
+            assert lib.tcb_op_rmsnorm(one[0, at:].data_ptr(), D, None, 0, None, 0, None, 1e-6, tb.BF16, z[k:].data_ptr(), D,
+                                      tb.E4M3, _p(s), group, 1, D, _stream()) == 0
+            assert torch.equal(z[k:k + D], y[r].view(torch.uint8)) and torch.equal(s[0], sc[r])
+
+
+def test_rmsnorm_sums_far_apart(lib):
+    """The residual's sum is rounded once, subnormals, infinities and sums past the type's end included."""
+    for dtype, vals in ((tb.BF16, [1e-40, 3e-39, 1.0, 257.0, 3e38, float("inf"), -0.0, 1e-3]),
+                        (tb.F16, [6e-8, 1e-6, 1.0, 2049.0, 65000.0, float("inf"), -0.0, 1e-3]),
+                        (tb.F32, [1e-44, 1e-39, 1.0, 16777217.0, 3e38, float("inf"), -0.0, 1e-3])):
+        v = torch.tensor(vals, device="cuda").to(TYPE[dtype])
+        x = torch.cat([v[:, None].expand(8, 8), v[:, None].expand(8, 8)], 1).contiguous()
+        r = torch.cat([v[None].expand(8, 8), -v[None].expand(8, 8)], 1).contiguous()
+        _, sm, _ = run_rms(lib, x, r, None, 16, dtype, dtype, 0)
+        want = (x.double() + r.double()).to(TYPE[dtype])
+        assert torch.equal(torch.isnan(sm), torch.isnan(want))
+        assert torch.equal(torch.nan_to_num(sm, 7.0), torch.nan_to_num(want, 7.0))
+
+
 def test_rmsnorm_without_eps(lib):
     """eps 0: rows far below 1 are normalised all the same; a row of zeros has no norm."""
     g = _gen(13)
