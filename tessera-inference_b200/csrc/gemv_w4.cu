@@ -26,7 +26,7 @@
 // the token rows of all K columns are too many for a block or the weight rows too
 // few for the SMs; the sums of the slices are joined over distributed shared memory.
 //
-// Measured (bf16 rows): 1 x 16,384 x 8,192 in 18.6 us, 3.7 TB/s of weights. Of that
+// Measured (bf16 rows): 1 x 16,384 x 8,192 in 18.3 us, 3.8 TB/s of weights. Of that
 // 2 us are the launch and 4 the code's first run and the token rows, while only the
 // rings fill; the records then stream at 5.5 TB/s (without any product: 16.7 us). 24
 // or 32 warps take 20 us, rings of four records 19.3. 8 x 8,192 x 8,192 in 15.8 us,
@@ -348,7 +348,9 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
         for (int step = 0; step < cut.steps && tile < tiles; ++step, tile += hop) {  // alike for all warps of a tile
             float acc[NT][4] = {};
             uint32_t xo = r0 * W4_COLS * 2, so = my_sums + r0 * (W4_COLS / SUB) * GROUP * 4;
-#pragma unroll 1
+            // two records' chains of products side by side, where the registers allow (one token on 16,384 x 8,192 with scales of
+            // 32: 23.4 us, one record at a time 25.1; with 32 tokens 36.7 and 36.0)
+#pragma unroll (NT == 1 ? 2 : 1)
             for (int r = 0; r < count; ++r) {
                 cp_async_wait<RING - 2>();
                 __syncwarp();
