@@ -201,7 +201,10 @@ __device__ __forceinline__ uint2 codes8(const float (&p)[8], const Step &s) {
 //   EDGED    the tensors' rows start equally far (o elements) behind such boundaries; the first and the last unit of a row
 //            are partly outside it and go element by element;
 //   SINGLE   nothing fits: value (i, j) is column (8 i + j) TEAM + t, one element per access, consecutive over a warp.
-enum RmsMode { ALIGNED, EDGED, SINGLE };
+//
+// ALIGNED_ROW is ALIGNED for codes with one scale per row: a kernel of its own, since the two kinds of scales together take
+// registers that rows of 2,560 columns and more miss (16,384: 151 us instead of 142).
+enum RmsMode { ALIGNED, EDGED, SINGLE, ALIGNED_ROW };
 
 // Threads of a block, and the registers of a thread, which bound the blocks on an SM: about what the packed row, and for
 // EDGED rows the row in f32, needs. Fewer spill, more leave HBM waiting (bf16 to e4m3, 524,288 x 640: 48 registers 396 us, 64
@@ -218,9 +221,9 @@ struct RmsShape {
 template <class T, class Y, int TEAM, int NU, RmsMode MODE>
 __global__ void __launch_bounds__(RmsShape<T, TEAM, NU, MODE>::THREADS, RmsShape<T, TEAM, NU, MODE>::BLOCKS) k_rmsnorm(const RmsArgs a) {
     constexpr int THREADS = RmsShape<T, TEAM, NU, MODE>::THREADS, ROWS = THREADS / TEAM;  // rows per block and pass
-    constexpr bool CODES = sizeof(Y) == 1;
+    constexpr bool CODES = sizeof(Y) == 1, BOUND = MODE == ALIGNED || MODE == ALIGNED_ROW;
     // units that the choice of the team leaves whole in aligned rows (a team of 512 with 4 units starts at 8,200 columns)
-    constexpr int FULL = MODE != ALIGNED || TEAM < 32 ? 0 : TEAM == 512 ? NU / 2 : NU - 1;
+    constexpr int FULL = !BOUND || TEAM < 32 ? 0 : TEAM == 512 ? NU / 2 : NU - 1;
     __shared__ float red[3][TEAM > 32 ? TEAM / 32 : 1];
     __shared__ uint32_t gtop[TEAM > 32 && MODE == SINGLE && CODES ? TEAM * NU * RMS_UNIT / 32 : 1];
     const int t = threadIdx.x % TEAM;
@@ -234,13 +237,13 @@ __global__ void __launch_bounds__(RmsShape<T, TEAM, NU, MODE>::THREADS, RmsShape
             return MODE == SINGLE ? (i * RMS_UNIT + j) * TEAM + t : (i * TEAM + t) * RMS_UNIT + j - o;
         };
         const auto whole = [&](int i) {
-            return MODE == ALIGNED ? i < FULL || col(i, 0) < D : MODE == EDGED && col(i, 0) >= 0 && col(i, 8) <= D;
+            return BOUND ? i < FULL || col(i, 0) < D : MODE == EDGED && col(i, 0) >= 0 && col(i, 8) <= D;
         };
         const auto in = [&](int i, int j) { return (MODE != EDGED || col(i, j) >= 0) && col(i, j) < D; };
         // unit i of a row that starts at p, zero outside the row; and back
         const auto get = [&](const T *p, int i) {
             Unit<T> u;
-            if (!(MODE == ALIGNED && i < FULL)) u.zero();
+            if (!(BOUND && i < FULL)) u.zero();
             if (whole(i)) u.load(p + col(i, 0));
             else if (MODE == SINGLE || (MODE == EDGED && col(i, 8) > 0 && col(i, 0) < D)) {
 #pragma unroll
@@ -288,7 +291,7 @@ __global__ void __launch_bounds__(RmsShape<T, TEAM, NU, MODE>::THREADS, RmsShape
         const auto weigh = [&](int i, float (&p)[8]) {
             h[i].get(p);
             if (!a.g) return;
-            if (MODE == ALIGNED) {
+            if (BOUND) {
                 if (whole(i)) {
                     const float4 u = __ldg(reinterpret_cast<const float4 *>(a.g + col(i, 0)));
                     const float4 w = __ldg(reinterpret_cast<const float4 *>(a.g + col(i, 0)) + 1);
@@ -380,7 +383,7 @@ __global__ void __launch_bounds__(RmsShape<T, TEAM, NU, MODE>::THREADS, RmsShape
                         if (in(i, j)) reinterpret_cast<uint8_t *>(y)[col(i, j)] = (uint8_t)((j < 4 ? q.x : q.y) >> 8 * (j % 4));
                 }
             };
-            if (a.group == 0) {
+            if (MODE == ALIGNED_ROW || (MODE != ALIGNED && a.group == 0)) {
                 float m = 0.f, p[NU][8];
 #pragma unroll
                 for (int i = 0; i < NU; ++i) {
@@ -391,7 +394,7 @@ __global__ void __launch_bounds__(RmsShape<T, TEAM, NU, MODE>::THREADS, RmsShape
                 if (t == 0 && D) scales[0] = s.s;
 #pragma unroll
                 for (int i = 0; i < NU; ++i) write(i, codes8<Y>(p[i], s));
-            } else if constexpr (MODE == ALIGNED || (MODE == EDGED && TEAM > 32)) {
+            } else if constexpr (BOUND || (MODE == EDGED && TEAM > 32)) {
                 // a group is 4, 8 or 16 neighbouring lanes, or the team (o = 0 here)
                 const int lanes = min(a.group / RMS_UNIT, TEAM);
 #pragma unroll
@@ -518,7 +521,7 @@ void rms_launch_team(const RmsArgs &a, cudaStream_t st) {
     if (units <= 32) return rms_launch<T, Y, 32, 1, MODE>(a, st);
     if constexpr (MODE != SINGLE) {
         if (units <= 64) return rms_launch<T, Y, 32, 2, MODE>(a, st);
-        if (MODE == ALIGNED && units <= 80) return rms_launch<T, Y, 16, 5, MODE>(a, st);
+        if ((MODE == ALIGNED || MODE == ALIGNED_ROW) && units <= 80) return rms_launch<T, Y, 16, 5, MODE>(a, st);
         if (units <= 96) return rms_launch<T, Y, 32, 3, MODE>(a, st);
     }
     if (units <= 128) return rms_launch<T, Y, 32, 4, MODE>(a, st);
@@ -541,7 +544,12 @@ template <class T>
 void rms_launch_type(const RmsArgs &a, int ytype, RmsMode mode, cudaStream_t st) {
     const auto by_mode = [&](auto y) {
         using Y = decltype(y);
-        if (mode == ALIGNED) rms_launch_team<T, Y, ALIGNED>(a, st);
+        if (mode == ALIGNED) {
+            if constexpr (sizeof(Y) == 1) {
+                if (a.group == 0) return rms_launch_team<T, Y, ALIGNED_ROW>(a, st);
+            }
+            rms_launch_team<T, Y, ALIGNED>(a, st);
+        }
         else if (mode == EDGED) rms_launch_team<T, Y, EDGED>(a, st);
         else rms_launch_team<T, Y, SINGLE>(a, st);
     };
