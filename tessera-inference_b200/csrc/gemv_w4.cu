@@ -26,7 +26,7 @@
 // the token rows of all K columns are too many for a block or the weight rows too
 // few for the SMs; the sums of the slices are joined over distributed shared memory.
 //
-// Measured (bf16 rows): 1 x 16,384 x 8,192 in 18.3 us, 3.8 TB/s of weights. Of that
+// Measured (bf16 rows): 1 x 16,384 x 8,192 in 18.1 us, 3.8 TB/s of weights. Of that
 // 2 us are the launch and 4 the code's first run and the token rows, while only the
 // rings fill; the records then stream at 5.5 TB/s (without any product: 16.7 us). 24
 // or 32 warps take 20 us, rings of four records 19.3. 8 x 8,192 x 8,192 in 15.8 us,
@@ -507,7 +507,8 @@ Fixed fixed_bytes(int ring, int group, int rows, int kb, int split, int sub, boo
 }
 
 // The cheapest cut by a model in clock cycles: a record takes an SM 46 cycles at HBM's rate or 32 per 8 token rows at
-// mma.sync's, and a warp 400 at least; a tile's end some 500, staging 2,000 and 24 bytes a cycle, a join the same again.
+// mma.sync's, and a warp 400 at least; a tile's end some 500, staging 2,000 and 24 bytes a cycle, a join twice that. Sizes only:
+// the cut sets the order of the sums, and pointers' alignment shall not.
 // Returns its cost, or INT64_MAX where nothing fits.
 int64_t best_cut(const W4Args &a, int mt, int ring, int sub, bool xg, int split, int blocks, W4Cut &out, int &bytes) {
     const int kb = (a.K + W4_COLS - 1) / W4_COLS, tiles = (a.N + W4_ROWS - 1) / W4_ROWS, nt = (out.rows + 7) / 8;
@@ -526,7 +527,7 @@ int64_t best_cut(const W4Args &a, int mt, int ring, int sub, bool xg, int split,
         }
         const int64_t count = ((kb + split - 1) / split + wk - 1) / wk;
         int64_t cost = std::max((int64_t)each * ((kb + split - 1) / split) * std::max(46, 32 * nt), batches * steps * count * 400);
-        cost += 2000 + f.x * (out.vec ? 1 : 2) / 24 + batches * steps * 500;
+        cost += 2000 + f.x / 24 + batches * steps * 500;
         if (split > 1) cost += batches * (4000 + (int64_t)steps * wt * tile_bytes / 24);
         if (cost >= best) continue;
         best = cost;

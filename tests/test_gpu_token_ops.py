@@ -553,7 +553,8 @@ def test_gemv_w4_largest(lib):
 @pytest.mark.parametrize("M,N,K,xtype", [(1, 40, 65536, tb.BF16), (9, 17, 65500, tb.F16), (3, 33, 40000, tb.E4M3),
                                          (33, 20, 16384, tb.BF16), (32, 4096, 8192, tb.BF16), (29, 700, 10001, tb.F16),
                                          (17, 8191, 5001, tb.I8), (300, 70, 700, tb.BF16), (1, 60000, 128, tb.BF16),
-                                         (5, 2000, 7000, tb.F16), (1, 256, 16384, tb.BF16)])
+                                         (5, 2000, 7000, tb.F16), (1, 256, 16384, tb.BF16),
+                                         (70000, 20, 130, tb.F16)])
 def test_gemv_w4_cuts(lib, M, N, K, xtype):
     """Sizes whose token rows or weight rows make the launch split K over clusters, slice a tile's records over warps, join in
     several batches, or cut the token rows."""
@@ -578,6 +579,22 @@ def test_gemv_w4_shifted_x(lib, shift, xtype):
                                   6, 50, 300, _stream()) == 0
         # whole numbers below 2^24 throughout: exact
         assert torch.equal(y.double(), x.double() @ codes.cuda().double().t() * (0.5 if xtype == tb.I8 else 1))
+
+
+def test_gemv_w4_same_bits_wherever_x_starts(lib):
+    g = _gen(21)
+    for M, N, K in ((1, 500, 4000), (17, 3000, 10001), (30, 100, 16384)):
+        codes = torch.randint(-8, 8, (N, K), generator=torch.Generator().manual_seed(4), dtype=torch.int8)
+        w = torch.from_numpy(tb.w4_pack(codes.numpy(), 128, np.full((N, -(-K // 128)), 0.01, np.float32))).cuda()
+        x0, ys = _randn(g, M, K).to(torch.bfloat16), []
+        for ld, shift in ((-(-K // 8) * 8, 0), (K + 1, 0), (K, 3)):
+            buf = torch.zeros(M * ld + 8, device="cuda", dtype=torch.bfloat16)
+            x = buf[shift:shift + M * ld].view(M, ld)
+            x[:, :K] = x0
+            ys.append(torch.zeros(M, N, device="cuda"))
+            assert lib.tcb_op_gemv_w4(buf[shift:].data_ptr(), ld, tb.BF16, None, 0, _p(w), 128, None, 0, None, 0, _p(ys[-1]), N,
+                                      tb.F32, M, N, K, _stream()) == 0
+        assert torch.equal(ys[0], ys[1]) and torch.equal(ys[0], ys[2])
 
 
 def test_gemv_w4_far_values(lib):
