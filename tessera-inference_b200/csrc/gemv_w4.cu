@@ -521,7 +521,7 @@ int64_t best_cut(const W4Args &a, int mt, int ring, int sub, bool xg, int split,
         int steps = (each + wt - 1) / wt, batches = 1;
         if (room < (split > 1 ? wt * tile_bytes : 0)) continue;
         if (split > 1) {
-            batches = (steps * wt * tile_bytes + room - 1) / room;
+            batches = (int)(((int64_t)steps * wt * tile_bytes + room - 1) / room);  // 2^31 bytes of sums and more at the largest N
             while ((steps + batches - 1) / batches * wt * tile_bytes > room) ++batches;
             steps = (steps + batches - 1) / batches;
         }

@@ -597,6 +597,24 @@ def test_gemv_w4_same_bits_wherever_x_starts(lib):
         assert torch.equal(ys[0], ys[1]) and torch.equal(ys[0], ys[2])
 
 
+@pytest.mark.parametrize("K", [1024, 2048])
+def test_gemv_w4_most_weight_rows(lib, K):
+    """2^24 weight rows with several tiles of 32 token rows: a cluster's sums for them all are 2^31 bytes. The weight rows
+    repeat, so the outputs have to, bit for bit."""
+    M, N, R = 320, 1 << 24, 64
+    codes = np.random.default_rng(5).integers(-8, 8, (R, K), dtype=np.int8)
+    w = torch.from_numpy(tb.w4_pack(codes, 128, np.full((R, K // 128), 0.0625, np.float32))).cuda().repeat(N // R)
+    x = _randn(_gen(22), M, K).to(torch.bfloat16)
+    y = torch.full((M, N), float("nan"), device="cuda", dtype=torch.bfloat16)
+    assert lib.tcb_op_gemv_w4(_p(x), K, tb.BF16, None, 0, _p(w), 128, None, 0, None, 0, _p(y), N, tb.BF16, M, N, K, _stream()) == 0
+    wd = torch.from_numpy(codes).cuda().double() * 0.0625
+    want, mag = x.double() @ wd.t(), x.double().abs() @ wd.abs().t()
+    sums = mag * (K + K / 16 + 16) * 2 * U
+    within(y[:, :R], want, sums + (want.abs() + sums) * HALF[tb.BF16] + TINY[tb.BF16])
+    for row in y:
+        assert torch.equal(row.view(-1, R), row[:R].expand(N // R, R))
+
+
 def test_gemv_w4_far_values(lib):
     """bf16 token rows of any size: each group is scaled by its largest value, which costs what is 2^-31 of it and smaller at
     most 2^-39 of it; the tolerance adds that times the weights' magnitudes. Sums are held times 2^-12 while subnormal steps
