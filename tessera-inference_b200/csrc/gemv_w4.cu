@@ -17,7 +17,8 @@
 // smaller by at most 2^-39 of it, far below what f32 sums of these terms round.
 // Products are exact and sums are f32; a group's sum is multiplied by its scale in
 // f32. An infinity or a NaN among the activations ends as NaN in X: where the result
-// is NaN, it is computed again from the definition, one product after the other.
+// is NaN, it is computed again from the definition, one product after the other; so is
+// what an infinite scale of x enters.
 //
 // One block of 16 warps per SM stays for the whole call. It keeps its token rows
 // in shared memory and streams weight records, each warp through a ring of its
@@ -197,7 +198,7 @@ __device__ __forceinline__ Beside beside(const W4Args &a, int otype, bool row_sc
 }
 __device__ __forceinline__ void put_out(const W4Args &a, int xtype, int otype, int m, int n, float v, const Beside &b) {
     v *= b.scale;
-    if (v != v) v = w4_plain(a, xtype, m, n);
+    if (v != v || isinf(b.scale)) v = w4_plain(a, xtype, m, n);
     v += b.bias;
     if (a.relu) v = v < 0.f ? 0.f : v;
     if (a.res) v += b.res;
@@ -333,6 +334,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
                 at[0] = at[2] = sum * (-8.f * 0x1p-24f);
                 if constexpr (XG) {
                     if (xtype != TCB_BF16) back = k0 + k < a.K ? __ldg(a.xscales + (int64_t)(m0 + m) * ((a.K + a.xgroup - 1) / a.xgroup) + (k0 + k) / a.xgroup) : 0.f;
+                    if (isinf(back)) back = __int_as_float(0x7fffffff);  // NaN: the signs are the definition's
                     at[4] = back * 0x1p12f;  // the other half of 2^24 at the tile's end, so that neither leaves f32's range
                 }
             }

@@ -676,6 +676,34 @@ def test_gemv_w4_nan_and_inf_stay_in_their_row(lib):
     assert torch.isnan(y[1]).all() and torch.isposinf(y[3]).all() and torch.isfinite(y[[0, 2, 4]]).all()
 
 
+@pytest.mark.parametrize("K, group, xgroup", [(2045, 32, 64), (131, 128, 32), (7, 64, 0)])
+def test_gemv_w4_infinity_in_the_last_column(lib, K, group, xgroup):
+    """Rows that end inside a step of columns: an infinite last value, or an infinite last scale of 8-bit rows."""
+    N, ng = 20, -(-K // group)
+    codes = np.random.default_rng(6).integers(1, 8, (N, K), dtype=np.int8)
+    codes[1, -1], codes[2, -1], codes[3] = 0, -3, -1
+    w = torch.from_numpy(tb.w4_pack(codes, group, np.ones((N, ng), np.float32))).cuda()
+    wd = torch.from_numpy(codes).cuda().double()
+
+    def check(x, xtype, xs, xd):
+        y = torch.zeros(2, N, device="cuda")
+        assert lib.tcb_op_gemv_w4(_p(x), K, xtype, _p(xs), xgroup if xs is not None else 0, _p(w), group, None, 0, None, 0,
+                                  _p(y), N, tb.F32, 2, N, K, _stream()) == 0
+        assert torch.equal(torch.nan_to_num(y.double(), 7, 8, 9), torch.nan_to_num(xd @ wd.t(), 7, 8, 9))
+
+    x = torch.ones(2, K, device="cuda")
+    x[1, -1] = float("inf")
+    for xtype in (tb.BF16, tb.F16):
+        xt = x.to(TYPE[xtype])
+        check(xt, xtype, None, xt.double())
+    per = xgroup or K
+    xs = torch.ones(2, -(-K // per), device="cuda")
+    xs[1, -1] = float("inf")
+    for xtype in (tb.I8, tb.E4M3):
+        xt = torch.ones(2, K, device="cuda").to(TYPE[xtype])
+        check(xt, xtype, xs, xt.double() * xs.double().repeat_interleave(per, 1)[:, :K])
+
+
 # ------------------------------------------------------------------ together
 def test_zero_rows_are_a_no_op(lib):
     x = torch.ones(64, device="cuda", dtype=torch.bfloat16)
