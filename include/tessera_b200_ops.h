@@ -174,9 +174,9 @@ int tcb_rope_freqs(int rot, double base, int scaling, double factor, double span
  * contiguous rows of ceil(K / xgroup); xgroup 0 = one per row, else 32, 64 or
  * 128): the output of tcb_op_rmsnorm. bias: N f32 or NULL. res (pitch ldr) has
  * the output's type and may be out itself. otype is TCB_BF16, TCB_F16 or
- * TCB_F32. Products are exact (bf16 values below 2^-31 of the largest in their
- * group are rounded by at most 2^-39 of it) and summed in f32 in an order that depends on
- * xtype, M, N, K, group, xgroup and the GPU's SMs only; the output is rounded once. The
+ * TCB_F32. Products are exact and summed in f32 in an order that depends on
+ * xtype, M, N, K, group, xgroup and the GPU's SMs only; the output is rounded
+ * once. A code of 0 adds 0, whatever finite value it meets. The
  * weights are read once per 32 rows or so, so for hundreds of rows tcb_op_gemm
  * on bf16 weights is the faster call. M <= 2^18, N <= 2^24, K <= 65536. */
 int tcb_op_gemv_w4(const void *x, int64_t ldx, int xtype, const float *xscales, int xgroup, const void *w, int group,

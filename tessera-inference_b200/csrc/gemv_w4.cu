@@ -5,20 +5,16 @@
 // its N side, and the weights' codes arrive in the order of its A operand. What has
 // to be cheap is turning codes into 16-bit floats:
 //
-//   u = q + 8 in the low bits of an fp16 is the subnormal u 2^-24, in bits 4-7 it is
-//   16 u 2^-24, both exact. So a logic instruction per pair, and a shift per eight
-//   codes, are all; the two kinds of pairs go to sums of their own, X and Y, and a
-//   group's sum is 2^24 (X + Y / 16) - 8 (sum of the group's x). The last term is
-//   the same for all weight rows: it is summed once per block and X starts with it.
+//   u = q + 8 in the low bits of a 16-bit float (fp16 or bf16, as the token rows) is the subnormal u e, in bits 4-7 it is
+//   16 u e, e the type's smallest step. One logic instruction per pair of codes brings it there (and one shift per eight), one
+//   fused multiply-add makes it q 2^-10: both exact, so a code of 0 is a 0 whatever x it meets.
 //
-// The token rows are staged as fp16. That is exact for fp16, int8 and e4m3. A group
-// of a bf16 row is scaled by a power of two that takes its largest finite value to
-// 2^14 or above, which is exact down to 2^-31 of that value and rounds what is
-// smaller by at most 2^-39 of it, far below what f32 sums of these terms round.
-// Products are exact and sums are f32; a group's sum is multiplied by its scale in
-// f32. An infinity or a NaN among the activations ends as NaN in X: where the result
-// is NaN, it is computed again from the definition, one product after the other; so is
-// what an infinite scale of x enters.
+// Products are exact, sums are f32; a group's sum is multiplied by its scale in f32. With the 2^-10 no group's sum leaves
+// f32's range, whatever bf16 values it has, and no product falls below its smallest step; the outputs are multiplied by 2^10.
+// Infinities and NaN among the activations take their course. Outputs of 8-bit x that
+// are NaN or have an infinite scale are computed again from the definition, where the scale meets each x and not their sum.
+//
+// bf16 and fp16 token rows are staged as they are, 8-bit ones as fp16, which holds them exactly.
 //
 // One block of 16 warps per SM stays for the whole call. It keeps its token rows
 // in shared memory and streams weight records, each warp through a ring of its
@@ -27,12 +23,10 @@
 // the token rows of all K columns are too many for a block or the weight rows too
 // few for the SMs; the sums of the slices are joined over distributed shared memory.
 //
-// Measured (bf16 rows): 1 x 16,384 x 8,192 in 18.1 us, 3.8 TB/s of weights. Of that
+// Measured (bf16 rows): 1 x 16,384 x 8,192 in 18.6 us, 3.7 TB/s of weights. Of that
 // 2 us are the launch and 4 the code's first run and the token rows, while only the
-// rings fill; the records then stream at 5.5 TB/s (without any product: 16.7 us). 24
-// or 32 warps take 20 us, rings of four records 19.3. 8 x 8,192 x 8,192 in 15.8 us,
-// 32 x 8,192 x 8,192 in 35.7: with more token rows the staging, its codes' sums and
-// the join take most of the time, the products 10 us. 1 x 2,560 x 1,280 in 4.8 us.
+// rings fill. 8 x 8,192 x 8,192 in 15.0 us, 32 x 8,192 x 8,192 in 30.4, 1 x 2,560 x
+// 1,280 in 4.8 us.
 #include <algorithm>
 #include <atomic>
 
@@ -44,30 +38,54 @@ namespace tcb {
 namespace {
 
 constexpr int W4_WARPS = 16, W4_THREADS = W4_WARPS * 32;
+constexpr int RING = 4;    // records in flight per warp; eight are faster by 2% at most on 46 sizes, and take room
 constexpr int X_PAD = 32;  // 16-bit elements behind a staged token row: rows start 16 banks apart
 constexpr int SMEM_MAX = 227 * 1024;
 
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// d = A B + c on bf16 (BF) or fp16
+template <bool BF>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float4 c) {
+    if constexpr (BF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
 }
 
-// the same from c, or from zero
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float4 c) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
+// Two codes u = q + 8, in the low bits of a word's halves (HIGH: in their bits 4-7), as q 2^-10.
+constexpr float W4_CODE = 0x1p-10f;
+template <bool BF, bool HIGH>
+__device__ __forceinline__ uint32_t codes2(uint32_t u) {
+    constexpr float UP = (BF ? 0x1p123f : 0x1p14f) / (HIGH ? 16.f : 1.f);  // 2^-10 over the type's smallest step
+    uint32_t w;
+    if constexpr (BF) {
+        const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&u), __float2bfloat162_rn(UP), __float2bfloat162_rn(-8.f * W4_CODE));
+        memcpy(&w, &v, 4);
+    } else {
+        const __half2 v = __hfma2(*reinterpret_cast<const __half2 *>(&u), __float2half2_rn(UP), __float2half2_rn(-8.f * W4_CODE));
+        memcpy(&w, &v, 4);
+    }
+    return w;
+}
+
+// An 8-bit element of x, or two, as fp16.
+__device__ __forceinline__ uint16_t half_of(uint8_t v, int xtype) {
+    if (xtype == TCB_I8) return __half_as_ushort(__short2half_rn((int8_t)v));
+    return __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)v, __NV_E4M3).x;
+}
+__device__ __forceinline__ uint32_t half2_of(uint32_t v, int xtype) {
+    __half2 h;
+    if (xtype == TCB_I8) h = __floats2half2_rn((float)(int8_t)v, (float)(int8_t)(v >> 8));
+    else h = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v & 0xffffu), __NV_E4M3));
+    return *reinterpret_cast<const uint32_t *>(&h);
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t p) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
-    return v;
-}
-__device__ __forceinline__ float4 lds_f32x4(uint32_t p) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(p) : "memory");
     return v;
 }
 __device__ __forceinline__ float2 lds_f32x2(uint32_t p) {
@@ -112,9 +130,9 @@ struct Pass {
 };
 
 // A warp's passes of `rows` rows of x into shared memory, N passes' loads at once. `left`: columns of x
-// from its first one here on; the rest up to kn are zero.
+// from its first one here on; the rest up to kn are zero. 8-bit elements become fp16.
 template <int N, class E>
-__device__ __forceinline__ void x_scatter(const E *x, int64_t ldx, int left, int kn, int rows, uint16_t *xs, int pitch) {
+__device__ __forceinline__ void x_scatter(const E *x, int xtype, int64_t ldx, int left, int kn, int rows, uint16_t *xs, int pitch) {
     const int lane = threadIdx.x & 31;
     Pass load((kn + 255) / 256, threadIdx.x >> 5), put = load;
 #pragma unroll 1
@@ -132,7 +150,7 @@ __device__ __forceinline__ void x_scatter(const E *x, int64_t ldx, int left, int
             const int c = put.p * 256 + lane, end = put.m < rows ? kn : 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (c + 32 * j < end) xs[put.m * pitch + c + 32 * j] = (uint16_t)u[i][j];
+                if (c + 32 * j < end) xs[put.m * pitch + c + 32 * j] = sizeof(E) == 1 ? half_of((uint8_t)u[i][j], xtype) : (uint16_t)u[i][j];
         }
     }
 }
@@ -143,39 +161,43 @@ __device__ __forceinline__ void x_scatter(const E *x, int64_t ldx, int left, int
 struct W4Cut {
     int split = 1, wk = 1, clusters = 1, steps = 1, batches = 1;
     int rows = 1;                                                    // token rows of a full tile
-    int x_at = 0, sums_at = 0, red_at = 0, part_at = 0;              // byte offsets in shared memory
+    int x_at = 0, xs_at = 0, red_at = 0, part_at = 0;                // byte offsets in shared memory
     bool vec = false;                                                // x rows can be read in 8-element steps
 };
 
-// Output (m, n) from the definition, for results that are NaN. Stops where the sum is NaN for good, so that a padding row of NaN
-// costs next to nothing (32 x 8,192 x 8,192 with one: 42 us, without the stop 7.4 ms); a single infinity takes the whole row, 3.1 ms.
-__device__ __noinline__ float w4_plain(const W4Args &a, int xtype, int64_t m, int n) {
-    const int kb = (a.K + W4_COLS - 1) / W4_COLS, rec = w4_record_bytes(a.group), r = n % W4_ROWS;
+// Outputs (m, n) of 8-bit x from the definition, for the lanes that ask: all lanes of the warp come here and sum one output after
+// the other, in f64, where every product is exact. Stops where the sum is NaN for good, so that a padding row of NaN costs
+// little.
+__device__ __noinline__ float w4_plain(const W4Args &a, int xtype, bool ask, int m, int n, float v) {
+    const int lane = threadIdx.x & 31, kb = (a.K + W4_COLS - 1) / W4_COLS, rec = w4_record_bytes(a.group);
     const int xg = a.xgroup ? a.xgroup : a.K, nxg = (a.K + xg - 1) / xg;
-    const uint8_t *w = static_cast<const uint8_t *>(a.w) + (int64_t)(n / W4_ROWS) * kb * rec;
-    const int64_t row = m * a.ldx;
-    float v = 0.f;
+    for (uint32_t asked = __ballot_sync(~0u, ask); asked; asked &= asked - 1) {
+        const int who = __ffs(asked) - 1, row = __shfl_sync(~0u, m, who), r = __shfl_sync(~0u, n, who);
+        const uint8_t *w = static_cast<const uint8_t *>(a.w) + (int64_t)(r / W4_ROWS) * kb * rec;
+        const int half = r % W4_ROWS / 8, low = r % 8;
+        double sum = 0.;
 #pragma unroll 1
-    for (int k0 = 0; k0 < a.K && v == v; k0 += 8) {  // 8 columns: one word of codes, one scale; a sum that is NaN stays NaN
-        const int j = k0 % W4_COLS, i = j / 32, t = j / 8 % 4;
-        const uint8_t *p = w + (int64_t)(k0 / W4_COLS) * rec;
-        const uint32_t codes = *reinterpret_cast<const uint32_t *>(p + 512 * (r / 8) + 64 * (r % 8) + 16 * t + 4 * i);
-        const float s = to_f32(reinterpret_cast<const bf16 *>(p + W4_CODE_BYTES)[j / a.group * W4_ROWS + r]);
-        const float xs = a.xscales ? a.xscales[m * nxg + k0 / xg] : 1.f;
-        float x[8];
+        for (int first = 0; first < a.K; first += 256) {
+            const int k0 = first + lane * 8;  // 8 columns: one word of codes, one scale of each kind
+            if (k0 < a.K) {
+                const int j = k0 % W4_COLS, i = j / 32, t = j / 8 % 4;
+                const uint8_t *p = w + (int64_t)(k0 / W4_COLS) * rec;
+                const uint32_t codes = *reinterpret_cast<const uint32_t *>(p + 512 * half + 64 * low + 16 * t + 4 * i);
+                const double s = to_f32(reinterpret_cast<const bf16 *>(p + W4_CODE_BYTES)[j / a.group * W4_ROWS + r % W4_ROWS]);
+                const double xs = a.xscales[(int64_t)row * nxg + k0 / xg];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            const int64_t at = row + min(k0 + c, a.K - 1);
-            if (xtype == TCB_BF16) x[c] = to_f32(static_cast<const bf16 *>(a.x)[at]);
-            else if (xtype == TCB_F16) x[c] = to_f32(static_cast<const f16 *>(a.x)[at]);
-            else if (xtype == TCB_I8) x[c] = to_f32(static_cast<const int8_t *>(a.x)[at]);
-            else x[c] = to_f32(static_cast<const e4m3 *>(a.x)[at]);
+                for (int c = 0; c < 8; ++c)
+                    if (k0 + c < a.K) {
+                        const int64_t at = row * a.ldx + k0 + c;
+                        const float x = xtype == TCB_I8 ? to_f32(static_cast<const int8_t *>(a.x)[at]) : to_f32(static_cast<const e4m3 *>(a.x)[at]);
+                        sum += x * xs * ((int)(codes >> 4 * (c / 2 + 4 * (c % 2)) & 15) - 8) * s;
+                    }
+            }
+            if (__any_sync(~0u, sum != sum)) break;
         }
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            const int q = (int)(codes >> 4 * (c / 2 + 4 * (c % 2)) & 15) - 8;
-            if (k0 + c < a.K) v += x[c] * xs * (float)q * s;
-        }
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        if (lane == who) v = (float)sum;
     }
     return v;
 }
@@ -196,9 +218,16 @@ __device__ __forceinline__ Beside beside(const W4Args &a, int otype, bool row_sc
     }
     return b;
 }
-__device__ __forceinline__ void put_out(const W4Args &a, int xtype, int otype, int m, int n, float v, const Beside &b) {
-    v *= b.scale;
-    if (v != v || isinf(b.scale)) v = w4_plain(a, xtype, m, n);
+// Writes the outputs of a warp's lanes that have one; all lanes come here.
+template <bool CODES>
+__device__ __forceinline__ void put_out(const W4Args &a, int xtype, int otype, bool out, int m, int n, float v, const Beside &b) {
+    v *= 1.f / W4_CODE;
+    if (CODES && a.xscales) {
+        v *= b.scale;
+        const bool ask = out && (v != v || isinf(b.scale));
+        if (__any_sync(~0u, ask)) v = w4_plain(a, xtype, ask, m, n, v);
+    }
+    if (!out) return;
     v += b.bias;
     if (a.relu) v = v < 0.f ? 0.f : v;
     if (a.res) v += b.res;
@@ -208,9 +237,10 @@ __device__ __forceinline__ void put_out(const W4Args &a, int xtype, int otype, i
     else static_cast<float *>(a.out)[at] = v;
 }
 
-// SUB: columns whose products share both scales. NT: tiles of 8 token rows. XG: x has scales that change along a row, the
-// caller's or those of staged bf16. RING: records in flight per warp.
-template <int SUB, int NT, bool XG, int RING>
+// SUB: columns whose products share both scales. NT: tiles of 8 token rows. X: bf16 x, fp16 x (or 8-bit with one scale per row),
+// or 8-bit x with scales along its rows.
+enum W4X { X_BF16, X_F16, X_SCALED };
+template <int SUB, int NT, W4X X>
 __global__ void __launch_bounds__(W4_THREADS, 1)
     k_gemv_w4(const __grid_constant__ W4Args a, const __grid_constant__ W4Cut cut, const int xtype, const int otype) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -267,77 +297,31 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
     for (int s = 2; s < RING - 1; ++s) fetch(ring + s * rec + lane * 16);
 
     uint16_t *xs = reinterpret_cast<uint16_t *>(smem + cut.x_at);
-    // per group and pair of token rows: the pair's sums, twice (what X starts with), then its scales
-    float *sums = reinterpret_cast<float *>(smem + cut.sums_at);
-    constexpr int PAIR = XG ? 8 : 4, GROUP = 4 * NT * PAIR;
     if (!cut.vec) {
-        // rows that no vector fits: one element per access, consecutive over the warp, to their places first (8-bit ones as 16)
-        if (wide) x_scatter<4>(static_cast<const uint16_t *>(a.x) + (int64_t)m0 * a.ldx + k0, a.ldx, a.K - k0, kn, rows, xs, pitch);
-        else x_scatter<4>(static_cast<const uint8_t *>(a.x) + (int64_t)m0 * a.ldx + k0, a.ldx, a.K - k0, kn, rows, xs, pitch);
-        __syncwarp();
-    }
+        // rows that no vector fits: one element per access, consecutive over the warp
+        if (wide) x_scatter<4>(static_cast<const uint16_t *>(a.x) + (int64_t)m0 * a.ldx + k0, xtype, a.ldx, a.K - k0, kn, rows, xs, pitch);
+        else x_scatter<4>(static_cast<const uint8_t *>(a.x) + (int64_t)m0 * a.ldx + k0, xtype, a.ldx, a.K - k0, kn, rows, xs, pitch);
+    } else {
 #pragma unroll 1
-    for (; go.m < rows; go.next()) {
-        uint4 v = ahead[0];
-        ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = ahead[3];
-        ahead[3] = x_load();
-        const int m = go.m, k = go.p * 256 + lane * 8;
-        if (!cut.vec) {
-            v = k < kn ? *reinterpret_cast<const uint4 *>(xs + m * pitch + k) : make_uint4(0, 0, 0, 0);
-            if (!wide)
-                v = make_uint4((v.x & 0xffu) | (v.x >> 8 & 0xff00u) | v.y << 16 & 0xff0000u | (v.y << 8 & 0xff000000u),
-                               (v.z & 0xffu) | (v.z >> 8 & 0xff00u) | v.w << 16 & 0xff0000u | (v.w << 8 & 0xff000000u), 0, 0);
+        for (; go.m < rows; go.next()) {
+            uint4 v = ahead[0];
+            ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = ahead[3];
+            ahead[3] = x_load();
+            const int k = go.p * 256 + lane * 8;
+            if (!wide) v = make_uint4(half2_of(v.x, xtype), half2_of(v.x >> 16, xtype), half2_of(v.y, xtype), half2_of(v.y >> 16, xtype));
+            if (k < kn) *reinterpret_cast<uint4 *>(xs + go.m * pitch + k) = v;
         }
-        uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        float f[8], back = 1.f;
-        if (xtype == TCB_BF16) {
-            uint32_t top = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t lo = w[j] << 16 & 0x7fff0000u, hi = w[j] & 0x7fff0000u;
-                top = max(top, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
-            }
-#pragma unroll
-            for (int o = 1; o < SUB / 8; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
-            // 2^(14 - exponent of the largest value), in two factors that f32 holds; back is its inverse
-            const int up = 14 - max((int)(top >> 23) - 127, -126);
-            const float f0 = __uint_as_float((uint32_t)(up / 2 + 127) << 23), f1 = __uint_as_float((uint32_t)(up - up / 2 + 127) << 23);
-            back = __uint_as_float((uint32_t)(127 - up / 2) << 23) * __uint_as_float((uint32_t)(127 - up + up / 2) << 23);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const __half2 h = __floats2half2_rn(bf16lo(w[j]) * f0 * f1, bf16hi(w[j]) * f0 * f1);
-                w[j] = *reinterpret_cast<const uint32_t *>(&h);
-            }
-        } else if (!wide) {
-#pragma unroll
-            for (int j = 3; j >= 0; --j) {
-                const uint32_t b = w[j / 2] >> 16 * (j % 2) & 0xffffu;
-                __half2 h;
-                if (xtype == TCB_I8) h = __floats2half2_rn((float)(int8_t)b, (float)(int8_t)(b >> 8));
-                else h = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)b, __NV_E4M3));
-                w[j] = *reinterpret_cast<const uint32_t *>(&h);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
-            f[2 * j] = h.x;
-            f[2 * j + 1] = h.y;
-        }
-        float sum = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
-#pragma unroll
-        for (int o = 1; o < SUB / 8; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
-        if (k < kn) {
-            *reinterpret_cast<uint4 *>(xs + m * pitch + k) = make_uint4(w[0], w[2], w[1], w[3]);  // X's half, then Y's
-            if (k % SUB == 0) {
-                float *at = sums + k / SUB * GROUP + m / 2 * PAIR + m % 2;
-                at[0] = at[2] = sum * (-8.f * 0x1p-24f);
-                if constexpr (XG) {
-                    if (xtype != TCB_BF16) back = k0 + k < a.K ? __ldg(a.xscales + (int64_t)(m0 + m) * ((a.K + a.xgroup - 1) / a.xgroup) + (k0 + k) / a.xgroup) : 0.f;
-                    if (isinf(back)) back = __int_as_float(0x7fffffff);  // NaN: the signs are the definition's
-                    at[4] = back * 0x1p12f;  // the other half of 2^24 at the tile's end, so that neither leaves f32's range
-                }
-            }
+    }
+    // x's scales, per SUB columns and pair of token rows
+    float *xsc = reinterpret_cast<float *>(smem + cut.xs_at);
+    constexpr bool XG = X == X_SCALED;
+    constexpr int GROUP = 8 * NT;
+    if constexpr (XG) {
+        const int subs = kn / SUB, nxg = (a.K + a.xgroup - 1) / a.xgroup;
+        for (int e = threadIdx.x; e < rows * subs; e += W4_THREADS) {
+            const int m = e / subs, j = e - m * subs, k = k0 + j * SUB;
+            const float s = k < a.K ? __ldg(a.xscales + (int64_t)(m0 + m) * nxg + k / a.xgroup) : 0.f;
+            xsc[j * GROUP + m] = isinf(s) ? __int_as_float(0x7fffffff) : s;  // NaN: the signs are the definition's
         }
     }
     __syncthreads();
@@ -345,7 +329,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
     uint32_t brow[NT];  // lanes behind the last token row read it again; their sums are not written
 #pragma unroll
     for (int n = 0; n < NT; ++n) brow[n] = smem_u32(xs) + (min(8 * n + g, rows - 1) * pitch + 8 * t) * 2;
-    const uint32_t my_sums = smem_u32(sums) + PAIR * 4 * t;
+    const uint32_t my_xsc = smem_u32(xsc) + 8 * t;
     float *red = reinterpret_cast<float *>(smem + cut.red_at), *part = reinterpret_cast<float *>(smem + cut.part_at);
     const int tile_floats = rows * W4_ROWS;
     namespace cg = cooperative_groups;
@@ -358,7 +342,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
 #pragma unroll 1
         for (int step = 0; step < cut.steps && tile < tiles; ++step, tile += hop) {  // alike for all warps of a tile
             float acc[NT][4] = {};
-            uint32_t xo = r0 * W4_COLS * 2, so = my_sums + r0 * (W4_COLS / SUB) * GROUP * 4;
+            uint32_t xo = r0 * W4_COLS * 2, so = my_xsc + r0 * (W4_COLS / SUB) * GROUP * 4;
             // two records' chains of products side by side, where the registers allow (one token on 16,384 x 8,192 with scales of
             // 32: 23.4 us, one record at a time 25.1; with 32 tokens 36.7 and 36.0)
 #pragma unroll (NT == 1 ? 2 : 1)
@@ -377,38 +361,33 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
                 before = slot;
                 slot = slot + rec == ring_end ? ring : slot + rec;
                 const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
-                float X[NT][4], Y[NT][4];
+                float v[NT][4];  // sums of SUB columns
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int sub = j * 32 / SUB;
                     const uint32_t vl = wl[j] >> 8, vh = wh[j] >> 8;
-                    const uint32_t A[4] = {wl[j] & 0x000f000fu, wh[j] & 0x000f000fu, vl & 0x000f000fu, vh & 0x000f000fu};
-                    const uint32_t B[4] = {wl[j] & 0x00f000f0u, wh[j] & 0x00f000f0u, vl & 0x00f000f0u, vh & 0x00f000f0u};
+                    constexpr bool BF = X == X_BF16;
+                    const uint32_t A[4] = {codes2<BF, false>(wl[j] & 0x000f000fu), codes2<BF, false>(wh[j] & 0x000f000fu),
+                                           codes2<BF, true>(wl[j] & 0x00f000f0u), codes2<BF, true>(wh[j] & 0x00f000f0u)};
+                    const uint32_t B[4] = {codes2<BF, false>(vl & 0x000f000fu), codes2<BF, false>(vh & 0x000f000fu),
+                                           codes2<BF, true>(vl & 0x00f000f0u), codes2<BF, true>(vh & 0x00f000f0u)};
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         const uint4 b = lds128(brow[n] + xo + 64 * j);
-                        if (j * 32 % SUB == 0) {
-                            mma16816(X[n], A, b.x, b.y, lds_f32x4(so + (sub * GROUP + 4 * n * PAIR) * 4));
-                            mma16816(Y[n], B, b.z, b.w, make_float4(0.f, 0.f, 0.f, 0.f));
-                        } else {
-                            mma16816(X[n], A, b.x, b.y);
-                            mma16816(Y[n], B, b.z, b.w);
-                        }
+                        mma16816<BF>(v[n], A, b.x, b.y, j * 32 % SUB == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v[n][0], v[n][1], v[n][2], v[n][3]));
+                        mma16816<BF>(v[n], B, b.z, b.w, make_float4(v[n][0], v[n][1], v[n][2], v[n][3]));
                     }
                     if ((j + 1) * 32 % SUB == 0) {
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            float v[4];
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) v[c] = fmaf(Y[n][c], 0.0625f, X[n][c]);
                             if constexpr (XG) {
-                                const float2 xf = lds_f32x2(so + (sub * GROUP + 4 * n * PAIR + 4) * 4);
-                                v[0] *= xf.x, v[1] *= xf.y, v[2] *= xf.x, v[3] *= xf.y;
+                                const float2 xf = lds_f32x2(so + (sub * GROUP + 8 * n) * 4);
+                                v[n][0] *= xf.x, v[n][1] *= xf.y, v[n][2] *= xf.x, v[n][3] *= xf.y;
                             }
-                            acc[n][0] = fmaf(v[0], su[sub], acc[n][0]);
-                            acc[n][1] = fmaf(v[1], su[sub], acc[n][1]);
-                            acc[n][2] = fmaf(v[2], sv[sub], acc[n][2]);
-                            acc[n][3] = fmaf(v[3], sv[sub], acc[n][3]);
+                            acc[n][0] = fmaf(v[n][0], su[sub], acc[n][0]);
+                            acc[n][1] = fmaf(v[n][1], su[sub], acc[n][1]);
+                            acc[n][2] = fmaf(v[n][2], sv[sub], acc[n][2]);
+                            acc[n][3] = fmaf(v[n][3], sv[sub], acc[n][3]);
                         }
                     }
                 }
@@ -426,32 +405,35 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {  // weight row g + 8 (c / 2), token row 8 n + 2 t + c % 2
                     const int m = 8 * n + 2 * t + c % 2;
-                    if (m < rows) buf[m * W4_ROWS + g + c / 2 * 8] = acc[n][c] * (XG ? 0x1p12f : 0x1p24f);
+                    if (m < rows) buf[m * W4_ROWS + g + c / 2 * 8] = acc[n][c];
                 }
             if (cut.wk > 1) asm volatile("bar.sync %0, %1;" ::"r"(my_t + 1), "r"(cut.wk * 32) : "memory");
             else __syncwarp();
             if (cut.wk == 1 && cut.split > 1) continue;
             buf -= my_k * tile_floats;
 #pragma unroll 1
-            for (int e = my_k * 32 + lane; e < tile_floats; e += cut.wk * 32) {
-                const int m = m0 + e / W4_ROWS, n = tile * W4_ROWS + e % W4_ROWS;
-                const bool out = cut.split == 1 && n < a.N;
+            for (int e0 = my_k * 32; e0 < tile_floats; e0 += cut.wk * 32) {  // a warp's lanes stay together
+                const int e = e0 + lane, m = m0 + e / W4_ROWS, n = tile * W4_ROWS + e % W4_ROWS;
+                const bool mine = e < tile_floats, out = mine && cut.split == 1 && n < a.N;
                 Beside b = {};
                 if (out) b = beside(a, otype, !XG && a.xscales, m, n);
                 float v = 0.f;
-                for (int k = 0; k < cut.wk; ++k) v += buf[k * tile_floats + e];
-                if (cut.split > 1) joined[e] = v;
-                else if (out) put_out(a, xtype, otype, m, n, v, b);
+                if (mine)
+                    for (int k = 0; k < cut.wk; ++k) v += buf[k * tile_floats + e];
+                if (cut.split > 1) {
+                    if (mine) joined[e] = v;
+                } else put_out<X != X_BF16>(a, xtype, otype, out, m, n, v, b);
             }
         }
         if (cut.split == 1) break;
         cl.sync();
         const int all = cut.steps * wt * tile_floats;
 #pragma unroll 1
-        for (int e = rank * W4_THREADS + threadIdx.x; e < all; e += 2 * cut.split * W4_THREADS) {
+        for (int e0 = rank * W4_THREADS + warp * 32; e0 < all; e0 += 2 * cut.split * W4_THREADS) {  // a warp's lanes stay together
+            const int e = e0 + lane;
             int m[2], n[2];
             float u[2][8];
-            Beside b[2];
+            Beside b[2] = {};
 #pragma unroll
             for (int i = 0; i < 2; ++i) {  // two outputs' loads, remote and global, before the first sum
                 const int f = e + i * cut.split * W4_THREADS, local = f / tile_floats, r = f - local * tile_floats;
@@ -468,7 +450,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
                 float v = 0.f;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v += u[i][k];
-                if (n[i] >= 0) put_out(a, xtype, otype, m[i], n[i], v, b[i]);
+                put_out<X != X_BF16>(a, xtype, otype, n[i] >= 0, m[i], n[i], v, b[i]);
             }
         }
         cl.sync();  // no block's sums go while another reads them
@@ -477,9 +459,9 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
 
 // Blocks that the device holds at once when every `split` of them form a cluster. Looked up once per device, as the kernel
 // gets its shared memory.
-template <int SUB, int NT, bool XG, int RING>
+template <int SUB, int NT, W4X X>
 int resident(int split) {
-    const auto kernel = k_gemv_w4<SUB, NT, XG, RING>;
+    const auto kernel = k_gemv_w4<SUB, NT, X>;
     static std::atomic<int> known[64][4];
     int dev = 0, n = 0;
     cudaGetDevice(&dev);
@@ -506,24 +488,26 @@ int resident(int split) {
     return std::max(n, split);
 }
 
-// Shared memory of the ring, and of `rows` token rows with their sums and scales in one of `split` slices.
+// Shared memory of the ring, and of `rows` token rows and their scales in one of `split` slices.
 struct Fixed {
-    int ring, x, sums;
-    int all() const { return ring + x + sums; }
+    int ring, x, scales;
+    int all() const { return ring + x + scales; }
 };
-Fixed fixed_bytes(int ring, int group, int rows, int kb, int split, int sub, bool xg) {
-    const int recs = (kb + split - 1) / split, pairs = (rows + 7) / 8 * 4;
-    return {W4_WARPS * ring * w4_record_bytes(group), rows * (recs * W4_COLS * 2 + X_PAD * 2),
-            pairs * recs * (W4_COLS / sub) * (xg ? 32 : 16)};
+Fixed fixed_bytes(int group, int rows, int kb, int split, int sub, bool xg) {
+    const int recs = (kb + split - 1) / split;
+    return {W4_WARPS * RING * w4_record_bytes(group), rows * (recs * W4_COLS * 2 + X_PAD * 2),
+            xg ? (rows + 7) / 8 * 8 * recs * (W4_COLS / sub) * 4 : 0};
 }
 
-// The cheapest cut by a model in clock cycles: a record takes an SM 46 cycles at HBM's rate or 32 per 8 token rows at
-// mma.sync's, and a warp 400 at least; a tile's end some 500, staging 2,000 and 24 bytes a cycle, a join twice that. Sizes only:
-// the cut sets the order of the sums, and pointers' alignment shall not.
+// The cheapest cut by a model in clock cycles: a record takes an SM 46 cycles at HBM's rate or 52 per 8 token rows (the codes'
+// way to 16 bits, the products, the fragments from shared memory), and a warp 500 and 200 per 8 token rows at least; a tile's
+// end 1,100, and 270 per slice that meets there, staging 2,000 and 9 bytes a cycle, a join 4,200. Fitted to every cut of 46
+// sizes of 1 to 64 token rows: what it takes is 0.7% slower than the best in the mean, 5.4% at most. Sizes only: the cut sets
+// the order of the sums, and pointers' alignment shall not.
 // Returns its cost, or INT64_MAX where nothing fits.
-int64_t best_cut(const W4Args &a, int mt, int ring, int sub, bool xg, int split, int blocks, W4Cut &out, int &bytes) {
+int64_t best_cut(const W4Args &a, int mt, int sub, bool xg, int split, int blocks, W4Cut &out, int &bytes) {
     const int kb = (a.K + W4_COLS - 1) / W4_COLS, tiles = (a.N + W4_ROWS - 1) / W4_ROWS, nt = (out.rows + 7) / 8;
-    const Fixed f = fixed_bytes(ring, a.group, out.rows, kb, split, sub, xg);
+    const Fixed f = fixed_bytes(a.group, out.rows, kb, split, sub, xg);
     const int tile_bytes = out.rows * W4_ROWS * 4, most = std::max(1, blocks / split / mt);
     int64_t best = INT64_MAX;
     for (int wk = 1; wk <= W4_WARPS && wk <= kb / split; wk *= 2) {
@@ -537,14 +521,14 @@ int64_t best_cut(const W4Args &a, int mt, int ring, int sub, bool xg, int split,
             steps = (steps + batches - 1) / batches;
         }
         const int64_t count = ((kb + split - 1) / split + wk - 1) / wk;
-        int64_t cost = std::max((int64_t)each * ((kb + split - 1) / split) * std::max(46, 32 * nt), batches * steps * count * 400);
-        cost += 2000 + f.x / 24 + batches * steps * 500;
-        if (split > 1) cost += batches * (4000 + (int64_t)steps * wt * tile_bytes / 24);
+        int64_t cost = std::max((int64_t)each * ((kb + split - 1) / split) * std::max(46, 52 * nt), batches * steps * count * (500 + 200 * nt));
+        cost += 2000 + f.x / 9 + (int64_t)batches * steps * (1100 + (wk > 1 ? 270 * wk : 0));
+        if (split > 1) cost += batches * 4200;
         if (cost >= best) continue;
         best = cost;
         out.split = split, out.wk = wk, out.clusters = clusters, out.steps = steps, out.batches = batches;
         out.x_at = f.ring;
-        out.sums_at = out.x_at + f.x;
+        out.xs_at = out.x_at + f.x;
         out.red_at = f.all();
         out.part_at = f.all() + red;
         bytes = out.part_at + (split > 1 ? steps * wt * tile_bytes : 0);
@@ -552,9 +536,9 @@ int64_t best_cut(const W4Args &a, int mt, int ring, int sub, bool xg, int split,
     return best;
 }
 
-template <int SUB, int NT, bool XG, int RING>
+template <int SUB, int NT, W4X X>
 void launch(const W4Args &a, const W4Cut &cut, int bytes, int mt, int xtype, int otype, cudaStream_t st) {
-    resident<SUB, NT, XG, RING>(1);
+    resident<SUB, NT, X>(1);
     cudaLaunchConfig_t c = {};
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -566,54 +550,47 @@ void launch(const W4Args &a, const W4Cut &cut, int bytes, int mt, int xtype, int
     c.stream = st;
     c.attrs = at;
     c.numAttrs = cut.split > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&c, k_gemv_w4<SUB, NT, XG, RING>, a, cut, xtype, otype);
+    const cudaError_t e = cudaLaunchKernelEx(&c, k_gemv_w4<SUB, NT, X>, a, cut, xtype, otype);
     need(e == cudaSuccess, cudaGetErrorString(e));
 }
 
-// Eight records in flight per warp cover what HBM holds back while the token rows are staged; four, where the token rows
-// leave no room for more.
-template <int SUB, int NT, bool XG>
+template <int SUB, int NT, W4X X>
 void launch_cut(const W4Args &a, int mt, int xtype, int otype, cudaStream_t st) {
     const int kb = (a.K + W4_COLS - 1) / W4_COLS;
     W4Cut base, cut;
     base.rows = (int)((a.M + (int64_t)mt - 1) / mt);
     base.vec = reinterpret_cast<uintptr_t>(a.x) % (xtype == TCB_I8 || xtype == TCB_E4M3 ? 8 : 16) == 0 && a.ldx % 8 == 0;
     int64_t best = INT64_MAX;
-    int bytes = 0, ring = 0;
-    for (int split = 1; split <= 8 && split <= kb; split *= 2)
-        for (int r = 8; r >= 4; r -= 4) {
-            W4Cut c = base;
-            int b = 0;
-            int64_t cost = best_cut(a, mt, r, SUB, XG, split, resident<SUB, NT, XG, 8>(split), c, b);
-            if (cost == INT64_MAX) continue;
-            if (r == 4) cost += cost / 8;
-            if (cost < best) best = cost, cut = c, bytes = b, ring = r;
-            break;
-        }
+    int bytes = 0;
+    for (int split = 1; split <= 8 && split <= kb; split *= 2) {
+        W4Cut c = base;
+        int b = 0;
+        const int64_t cost = best_cut(a, mt, SUB, X == X_SCALED, split, resident<SUB, NT, X>(split), c, b);
+        if (cost < best) best = cost, cut = c, bytes = b;
+    }
     need(best < INT64_MAX, "the token rows do not fit the shared memory");
-    if (ring == 8) launch<SUB, NT, XG, 8>(a, cut, bytes, mt, xtype, otype, st);
-    else launch<SUB, NT, XG, 4>(a, cut, bytes, mt, xtype, otype, st);
+    launch<SUB, NT, X>(a, cut, bytes, mt, xtype, otype, st);
 }
 
 // Token rows are cut into equal tiles of at most 32, and of no more than a cluster's shared memory holds.
-template <int SUB, bool XG>
+template <int SUB, W4X X>
 void launch_n(const W4Args &a, int xtype, int otype, cudaStream_t st) {
     const int kb = (a.K + W4_COLS - 1) / W4_COLS, split = kb >= 8 ? 8 : kb >= 4 ? 4 : kb >= 2 ? 2 : 1;
     int fit = 32;
-    while (fit > 1 && fixed_bytes(4, a.group, fit, kb, split, SUB, XG).all() + W4_WARPS * fit * W4_ROWS * 4 > SMEM_MAX) --fit;
+    while (fit > 1 && fixed_bytes(a.group, fit, kb, split, SUB, X == X_SCALED).all() + W4_WARPS * fit * W4_ROWS * 4 > SMEM_MAX) --fit;
     const int64_t mt = (a.M + fit - 1ll) / fit, rows = (a.M + mt - 1) / mt;
-    if (rows <= 8) launch_cut<SUB, 1, XG>(a, (int)mt, xtype, otype, st);
-    else if (rows <= 16) launch_cut<SUB, 2, XG>(a, (int)mt, xtype, otype, st);
-    else if (rows <= 24) launch_cut<SUB, 3, XG>(a, (int)mt, xtype, otype, st);
-    else launch_cut<SUB, 4, XG>(a, (int)mt, xtype, otype, st);
+    if (rows <= 8) launch_cut<SUB, 1, X>(a, (int)mt, xtype, otype, st);
+    else if (rows <= 16) launch_cut<SUB, 2, X>(a, (int)mt, xtype, otype, st);
+    else if (rows <= 24) launch_cut<SUB, 3, X>(a, (int)mt, xtype, otype, st);
+    else launch_cut<SUB, 4, X>(a, (int)mt, xtype, otype, st);
 }
 
-template <bool XG>
+template <W4X X>
 void launch_s(const W4Args &a, int xtype, int otype, cudaStream_t st) {
     const int sub = a.xgroup ? std::min(a.group, a.xgroup) : a.group;
-    if (sub == 32) launch_n<32, XG>(a, xtype, otype, st);
-    else if (sub == 64) launch_n<64, XG>(a, xtype, otype, st);
-    else launch_n<128, XG>(a, xtype, otype, st);
+    if (sub == 32) launch_n<32, X>(a, xtype, otype, st);
+    else if (sub == 64) launch_n<64, X>(a, xtype, otype, st);
+    else launch_n<128, X>(a, xtype, otype, st);
 }
 
 }  // namespace
@@ -635,8 +612,9 @@ void launch_gemv_w4(const W4Args &a, int xtype, int otype, cudaStream_t st) {
          "a pointer is not aligned to its elements");
     need(a.out != a.x, "out is x");
     need(a.res != a.out || !a.res || a.ldr == a.ldo || a.M == 1, "res is out with another pitch");
-    if (a.xgroup || xtype == TCB_BF16) launch_s<true>(a, xtype, otype, st);
-    else launch_s<false>(a, xtype, otype, st);
+    if (xtype == TCB_BF16) launch_s<X_BF16>(a, xtype, otype, st);
+    else if (!a.xgroup) launch_s<X_F16>(a, xtype, otype, st);
+    else launch_s<X_SCALED>(a, xtype, otype, st);
     check_token_launch("k_gemv_w4");
 }
 

@@ -704,6 +704,53 @@ def test_gemv_w4_infinity_in_the_last_column(lib, K, group, xgroup):
         check(xt, xtype, xs, xt.double() * xs.double().repeat_interleave(per, 1)[:, :K])
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 40, 1024), (3, 2048, 8192), (20, 64, 1000), (40, 100, 257)])
+@pytest.mark.parametrize("xtype,large,usual", [(tb.F16, 60000.0, 2e-3), (tb.F16, 1e3, 1e-3), (tb.BF16, 1e4, 1.0), (tb.BF16, 1e8, 1.0),
+                                               (tb.BF16, 1e30, 1.0), (tb.I8, 127.0, 1.0), (tb.E4M3, 448.0, 2.0 ** -6)])
+def test_gemv_w4_large_values_under_codes_of_zero(lib, M, N, K, xtype, large, usual):
+    """A large activation adds nothing where the code is 0: the bound stays that of the other terms' magnitudes, each
+    term and each sum rounded as elsewhere, and 99% of the results are within a few roundings."""
+    g, cols = _gen(23), [5, K // 2, K - 1]
+    for group, xgroup in ((128, 0), (32, 64)):
+        codes = torch.randint(-1, 2, (N, K), device="cuda", generator=g, dtype=torch.int8)
+        codes[::2, cols] = 0
+        codes[1::2, cols] = 1
+        w = torch.from_numpy(tb.w4_pack(codes.cpu().numpy(), group, np.ones((N, -(-K // group)), np.float32))).cuda()
+        x = usual * _randn(g, M, K)
+        x[:, cols] = torch.tensor([large, -large, large], device="cuda")
+        x, xs, per = (x.round() if xtype == tb.I8 else x).to(TYPE[xtype]), None, 0
+        xd = x.double()
+        if xtype in TOP:
+            per = xgroup
+            xs = 0.5 + torch.rand(M, -(-K // per) if per else 1, device="cuda", generator=g)
+            xd = xd * (xs.double().repeat_interleave(per, 1)[:, :K] if per else xs.double())
+        y = torch.zeros(M, N, device="cuda")
+        assert lib.tcb_op_gemv_w4(_p(x), K, xtype, _p(xs), per, _p(w), group, None, 0, None, 0, _p(y), N, tb.F32, M, N, K,
+                                  _stream()) == 0
+        wd = codes.double()
+        want, mag = xd @ wd.t(), xd.abs() @ wd.abs().t()
+        within(y, want, mag * (K + K / 16 + 16) * 2 * U + want.abs() * U)
+        assert ((y.double() - want).abs() <= want.abs() * 2 * U + mag * 16 * U).double().mean().item() >= 0.99
+
+
+@pytest.mark.parametrize("xtype", [tb.BF16, tb.F16, tb.I8, tb.E4M3])
+def test_gemv_w4_codes_of_zero(lib, xtype):
+    """All codes 0 under scales that are not: bias and residual and nothing else."""
+    g, N = _gen(24), 100
+    for M, K in ((1, 8192), (7, 700), (33, 2000)):
+        codes, ng = np.zeros((N, K), np.int8), -(-K // 64)
+        w = torch.from_numpy(tb.w4_pack(codes, 64, np.full((N, ng), 3.0, np.float32))).cuda()
+        x = 10 * _randn(g, M, K)
+        x = (x.round() if xtype == tb.I8 else x).to(TYPE[xtype])
+        xs = 0.5 + torch.rand(M, ng, device="cuda", generator=g) if xtype in TOP else None
+        b, r = _randn(g, N), _randn(g, M, N)
+        for bias, res in ((None, None), (b, r)):
+            y = torch.full((M, N), 77.0, device="cuda")
+            assert lib.tcb_op_gemv_w4(_p(x), K, xtype, _p(xs), 64 if xtype in TOP else 0, _p(w), 64, _p(bias), 0, _p(res), N, _p(y),
+                                      N, tb.F32, M, N, K, _stream()) == 0
+            assert torch.equal(y, torch.zeros(M, N, device="cuda") if bias is None else r + b)
+
+
 # ------------------------------------------------------------------ together
 def test_zero_rows_are_a_no_op(lib):
     x = torch.ones(64, device="cuda", dtype=torch.bfloat16)
