@@ -12,7 +12,8 @@
 // Products are exact, sums are f32; a group's sum is multiplied by its scale in f32. With the 2^-10 no group's sum leaves
 // f32's range, whatever bf16 values it has, and no product falls below its smallest step; the outputs are multiplied by 2^10.
 // Infinities and NaN among the activations take their course. Outputs of 8-bit x that
-// are NaN or have an infinite scale are computed again from the definition, where the scale meets each x and not their sum.
+// are not finite are computed again from the definition: a sum may leave f32's range before the scale that brings it back, and
+// an infinite scale meets each x there, not their sum.
 //
 // bf16 and fp16 token rows are staged as they are, 8-bit ones as fp16, which holds them exactly.
 //
@@ -224,7 +225,7 @@ __device__ __forceinline__ void put_out(const W4Args &a, int xtype, int otype, b
     v *= 1.f / W4_CODE;
     if (CODES && a.xscales) {
         v *= b.scale;
-        const bool ask = out && (v != v || isinf(b.scale));
+        const bool ask = out && !(fabsf(v) <= 3.4028235e38f);
         if (__any_sync(~0u, ask)) v = w4_plain(a, xtype, ask, m, n, v);
     }
     if (!out) return;
@@ -320,8 +321,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
         const int subs = kn / SUB, nxg = (a.K + a.xgroup - 1) / a.xgroup;
         for (int e = threadIdx.x; e < rows * subs; e += W4_THREADS) {
             const int m = e / subs, j = e - m * subs, k = k0 + j * SUB;
-            const float s = k < a.K ? __ldg(a.xscales + (int64_t)(m0 + m) * nxg + k / a.xgroup) : 0.f;
-            xsc[j * GROUP + m] = isinf(s) ? __int_as_float(0x7fffffff) : s;  // NaN: the signs are the definition's
+            xsc[j * GROUP + m] = k < a.K ? __ldg(a.xscales + (int64_t)(m0 + m) * nxg + k / a.xgroup) : 0.f;
         }
     }
     __syncthreads();

@@ -751,6 +751,33 @@ def test_gemv_w4_codes_of_zero(lib, xtype):
             assert torch.equal(y, torch.zeros(M, N, device="cuda") if bias is None else r + b)
 
 
+@pytest.mark.parametrize("xgroup", [0, 32, 64, 128])
+@pytest.mark.parametrize("xtype", [tb.I8, tb.E4M3])
+@pytest.mark.parametrize("xscale,wscale", [(2.0 ** 117, 2.0 ** -20), (2.0 ** 124, 2.0 ** -40), (2.0 ** -110, 2.0 ** 120), (2.0 ** 100, 2.0 ** 60)])
+def test_gemv_w4_far_scales(lib, xtype, xgroup, xscale, wscale):
+    """Finite scales of 8-bit rows, however far from 1: an output is finite where its sum is, and infinite where that is past
+    f32's end. A row of another scale beside them stays within the same bound."""
+    for M, N, K, group in ((3, 40, 384, 128), (9, 70, 4100, 32)):
+        g, nxg, ng = _gen(25), -(-K // xgroup) if xgroup else 1, -(-K // group)
+        codes = torch.randint(-8, 8, (N, K), device="cuda", generator=g, dtype=torch.int8)
+        codes[:4] = 7
+        w = torch.from_numpy(tb.w4_pack(codes.cpu().numpy(), group, np.full((N, ng), wscale, np.float32))).cuda()
+        x = TOP[xtype] * (1 - torch.rand(M, K, device="cuda", generator=g))
+        x[0, ::3] *= -1
+        x = (x.floor() if xtype == tb.I8 else x).to(TYPE[xtype])
+        xs = xscale * (1 - 0.5 * torch.rand(M, nxg, device="cuda", generator=g))
+        xs[2] = 0.5
+        y = torch.zeros(M, N, device="cuda")
+        assert lib.tcb_op_gemv_w4(_p(x), K, xtype, _p(xs), xgroup, _p(w), group, None, 0, None, 0, _p(y), N, tb.F32, M, N, K,
+                                  _stream()) == 0
+        xd = x.double() * xs.double().repeat_interleave(xgroup or K, 1)[:, :K]
+        wd = codes.double() * wscale
+        want, mag = xd @ wd.t(), xd.abs() @ wd.abs().t()
+        finite = mag < 2.0 ** 127
+        assert finite[:2].all() if xscale * wscale < 1e30 else (want[1].abs() > 2.0 ** 129).all()
+        within(y, want.to(torch.float32), mag * (K + K / 16 + 16) * 2 * U + want.abs() * U)
+
+
 # ------------------------------------------------------------------ together
 def test_zero_rows_are_a_no_op(lib):
     x = torch.ones(64, device="cuda", dtype=torch.bfloat16)
