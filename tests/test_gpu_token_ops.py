@@ -302,6 +302,21 @@ def test_rmsnorm_far_pitch(lib):
     check_rms(h, v, y, tb.E4M3, 0, sc)
 
 
+@pytest.mark.parametrize("D", [8, 640, 2560, 5001, 16384])
+@pytest.mark.parametrize("dtype", [tb.BF16, tb.F32])
+def test_rmsnorm_small_values_in_far_rows(lib, D, dtype):
+    """Rows whose squares overflow f32 keep every bit of their small values: each output is within the same relative bound."""
+    g = _gen(26)
+    x = _randn(g, 6, D) * torch.exp2(100 * torch.rand(6, D, device="cuda", generator=g) - 40)
+    x[:, 3] = torch.tensor([2.0 ** 70, 2.0 ** 80, 2.0 ** 64, 2.0 ** 100, 1.5 * 2.0 ** 127, 1.0], device="cuda")
+    x, w = x.to(TYPE[dtype]), 1 + 0.2 * _randn(g, D)
+    y, _, _ = run_rms(lib, x, None, w, D, dtype, dtype, 0)
+    _, v = rms_ref(x, None, w, 1e-6)
+    check_rms(None, v, y, dtype, 0, None)
+    z, _, sc = run_rms(lib, x, None, w, D, dtype, tb.E4M3, 32)
+    check_rms(None, v, z, tb.E4M3, 32, sc)
+
+
 # ------------------------------------------------------------------ rotary positions
 def rope_ref(x, pos, freq, mscale, rot, inter, inverse):
     """x: (M, heads, hd) f64; returns (out, magnitude of the two terms) in f64."""
