@@ -320,10 +320,11 @@ __global__ void __launch_bounds__(RmsShape<T, TEAM, NU, MODE>::THREADS, RmsShape
         };
         ss = team_sum<TEAM>(ss, red[0]);
         float eps = a.eps;
-        // Finite rows whose squares leave f32's range are scaled by a power of two first; fp16 rows never leave it. Large rows
+        // Finite rows whose squares leave f32's range (or do with eps) are scaled by a power of two first; fp16 rows never leave it. Large rows
         // come down until their largest value is 2^55 to 2^56, 16,384 squares of which f32 holds, and no further: what goes
         // below f32's and bf16's normal values there would do so in the output. Teams that share a warp go together.
-        const bool far = !std::is_same_v<T, f16> && (isinf(ss) || (ss < 0x1p-90f && eps < 0x1p-80f));
+        const bool over = isinf(fmaf(ss, a.inv_d, eps));
+        const bool far = !std::is_same_v<T, f16> && (over || (ss < 0x1p-90f && eps < 0x1p-80f));
         if (TEAM < 32 ? __any_sync(~0u, far) : far) {
             float m = 0.f;
 #pragma unroll
@@ -336,7 +337,7 @@ __global__ void __launch_bounds__(RmsShape<T, TEAM, NU, MODE>::THREADS, RmsShape
             if (TEAM > 32) __syncthreads();
             m = team_max<TEAM>(m, red[1]);
             const float down = __uint_as_float(min(309u - (__float_as_uint(m) >> 23), 119u) << 23);  // 2^(55 - m's exponent), at most 2^-8
-            const float pre = !far || !(m <= 3.4028235e38f) ? 1.f : isinf(ss) ? down : 0x1p100f;
+            const float pre = !far || !(m <= 3.4028235e38f) ? 1.f : over ? down : 0x1p100f;
             eps = eps * pre * pre;
             ss = 0.f;
 #pragma unroll

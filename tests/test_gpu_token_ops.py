@@ -317,6 +317,17 @@ def test_rmsnorm_small_values_in_far_rows(lib, D, dtype):
     check_rms(None, v, z, tb.E4M3, 32, sc)
 
 
+@pytest.mark.parametrize("dtype", [tb.BF16, tb.F32])
+def test_rmsnorm_largest_eps(lib, dtype):
+    """mean(h^2) + eps past f32's end, each within it."""
+    for D, h, eps in ((1, 1.8e19, 3e38), (2, 1.2e19, 3e38), (2, 1.2e19, 3.4e38), (64, 2.2e18, 3.39e38), (64, 1.0, 3.4e38), (1, 1e-20, 3.4e38)):
+        x = torch.full((3, D), h, device="cuda").to(TYPE[dtype])
+        x[1] *= -1
+        y, _, _ = run_rms(lib, x, None, None, D, dtype, dtype, 0, eps=eps)
+        _, v = rms_ref(x, None, None, float(np.float32(eps)))
+        check_rms(None, v, y, dtype, 0, None)
+
+
 # ------------------------------------------------------------------ rotary positions
 def rope_ref(x, pos, freq, mscale, rot, inter, inverse):
     """x: (M, heads, hd) f64; returns (out, magnitude of the two terms) in f64."""
