@@ -25,7 +25,7 @@ void launch_rmsnorm(RmsArgs a, int dtype, int ytype, cudaStream_t st) {
     need(apart(a.sum, a.lds, a.x, a.ldx) && apart(a.sum, a.lds, a.res, a.ldr) && apart(a.y, a.ldy, a.x, a.ldx) &&
              apart(a.y, a.ldy, a.sum, a.lds), "in place with another pitch");
     need(!codes || (a.y != a.x && a.y != a.res && a.y != a.sum), "8-bit output over its input");
-    need(a.y != a.res || !a.res, "y is res");
+    need(a.y != a.res || !a.res || a.sum == a.res, "y is res");  // but for y over sum over res
     a.inv_d = (float)(1.0 / a.D);
     a.shift = a.group == 128 ? 7 : a.group == 64 ? 6 : 5;
     // Where the rows start, in elements behind a boundary of 8: the same for every tensor, or one element at a time. Groups of

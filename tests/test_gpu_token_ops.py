@@ -328,6 +328,16 @@ def test_rmsnorm_largest_eps(lib, dtype):
         check_rms(None, v, y, dtype, 0, None)
 
 
+@pytest.mark.parametrize("D", [640, 641, 2560, 9001])
+def test_rmsnorm_all_over_res(lib, D):
+    """sum may be res and y may be sum, so y over res: the norm stands where the residual was."""
+    g = _gen(27)
+    x, r = _randn(g, 50, D).to(torch.bfloat16), _randn(g, 50, D).to(torch.bfloat16)
+    _, v = rms_ref(x, r, None, 1e-5)
+    assert lib.tcb_op_rmsnorm(_p(x), D, _p(r), D, _p(r), D, None, 1e-5, tb.BF16, _p(r), D, tb.BF16, None, 0, 50, D, _stream()) == 0
+    check_rms(None, v, r, tb.BF16, 0, None)
+
+
 # ------------------------------------------------------------------ rotary positions
 def rope_ref(x, pos, freq, mscale, rot, inter, inverse):
     """x: (M, heads, hd) f64; returns (out, magnitude of the two terms) in f64."""
