@@ -265,6 +265,10 @@ def w4_pack(w: np.ndarray, group: int, scales: np.ndarray | None = None) -> np.n
     """The packed 4-bit form of a weight matrix (N, K): tcb_w4_pack of f32
     weights, or tcb_w4_pack_codes of int8 codes in -8..7 with their scales."""
     lib = load_library()
+    if scales is not None:
+        w = np.asarray(w)
+        if not ((w >= -8) & (w <= 7) & (w == np.rint(w))).all():
+            raise ValueError("codes that are not whole numbers in -8..7")
     w = np.ascontiguousarray(w, np.float32 if scales is None else np.int8)
     N, K = w.shape
     n = lib.tcb_w4_bytes(N, K, group)

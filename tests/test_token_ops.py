@@ -197,3 +197,16 @@ def test_w4_pack_refusals(capfd):
     assert lib.tcb_w4_pack_codes(tb._ptr(codes), None, 1, 4, 32, tb._ptr(out)) == -1
     with pytest.raises(ValueError):
         tb.w4_pack(codes, 32, np.ones((1, 2), np.float32))
+
+
+@pytest.mark.parametrize("bad", [np.array([[0, 264, 0, 0]]), np.array([[0, -249, 0, 0]], np.int16), np.array([[0, 256, 0, 0]], np.uint16),
+                                 np.array([[0, 1.5, 0, 0]]), np.array([[0, np.nan, 0, 0]]), np.array([[0, 8, 0, 0]])])
+def test_w4_pack_codes_of_wider_types(bad):
+    """Codes that no int8 holds are refused and not wrapped into the range; whole ones in range are taken from any type."""
+    s = np.ones((1, 1), np.float32)
+    with pytest.raises(ValueError):
+        tb.w4_pack(bad, 32, s)
+    good = np.array([[-8, 7, 0, 3]])
+    want = tb.w4_pack(good.astype(np.int8), 32, s)
+    for t in (np.int64, np.int16, np.float32):
+        np.testing.assert_array_equal(tb.w4_pack(good.astype(t), 32, s), want)
