@@ -509,6 +509,28 @@ def test_rope_far_pitch(lib):
     within(x, want.to(torch.bfloat16), mag * 10 * U + want.abs() * 2.0 ** -7)
 
 
+def test_rope_f32_error(lib):
+    """f32 results in the root mean square, against cosines and sines rounded once from f64: what the fraction of a turn loses in
+    f32 is put back by one more rounding of each. That doubles their variance; the products' roundings are about as large and
+    stay: sqrt((2 + 1) / (1 + 1)) < 1.25."""
+    g, M, H, hd = _gen(28), 20000, 4, 128
+    x = _randn(g, M, H, hd)
+    x[:, 0, 64:], x[:, 1, :64] = 0, 0
+    pos = torch.randint(0, 4_000_000, (M,), device="cuda", generator=g, dtype=torch.int32)
+    freq, out = torch.from_numpy(tb.rope_freqs(hd)[0]).cuda(), torch.empty_like(x)
+    assert lib.tcb_op_rope(_p(x), H * hd, hd, tb.F32, _p(pos), 1, tb.I32, _p(freq), 1.0, hd, 0, 0, _p(out), H * hd, hd, M, H, hd,
+                           _stream()) == 0
+    want, mag = rope_ref(x.double(), pos, freq, 1.0, hd, False, False)
+    a = pos.double()[:, None] * freq
+    c, s, p, q = a.cos().float()[:, None], a.sin().float()[:, None], x[..., :64], x[..., 64:]
+    once = torch.cat([p * c - q * s, p * s + q * c], -1)
+
+    def rms(y):
+        return ((y.double() - want) / mag).square().mean().sqrt().item()
+
+    assert rms(out) <= 1.25 * rms(once)
+
+
 # ------------------------------------------------------------------ 4-bit product
 def w4_case(lib, M, N, K, group, xtype, otype, xgroup=0, relu=False, res=False, bias=True, pad=0, seed=0, in_place=False):
     g = _gen(seed + M + 3 * N + 5 * K)
