@@ -166,14 +166,35 @@ struct W4Cut {
     bool vec = false;                                                // x rows can be read in 8-element steps
 };
 
+// Whether a NaN is among a row's codes or scales; all lanes of a warp ask together.
+__device__ __forceinline__ bool nan_row(const W4Args &a, int xtype, int m) {
+    const int lane = threadIdx.x & 31, nxg = a.xgroup ? (a.K + a.xgroup - 1) / a.xgroup : 1;
+    bool found = false;
+    for (int g = lane; g < nxg; g += 32) found |= isnan(a.xscales[(int64_t)m * nxg + g]);
+    found = __any_sync(~0u, found);
+    const uint8_t *x = static_cast<const uint8_t *>(a.x) + m * a.ldx;
+    for (int k0 = 0; xtype == TCB_E4M3 && !found && k0 < a.K; k0 += 128) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) found |= (x[min(k0 + 32 * j + lane, a.K - 1)] & 0x7f) == 0x7f;
+        found = __any_sync(~0u, found);
+    }
+    return found;
+}
+
 // Outputs (m, n) of 8-bit x from the definition, for the lanes that ask: all lanes of the warp come here and sum one output after
-// the other, in f64, where every product is exact. Stops where the sum is NaN for good, so that a padding row of NaN costs
-// little.
+// the other, in f64, where every product is exact. Rows with a NaN, a padded batch's for instance, need no sum.
 __device__ __noinline__ float w4_plain(const W4Args &a, int xtype, bool ask, int m, int n, float v) {
     const int lane = threadIdx.x & 31, kb = (a.K + W4_COLS - 1) / W4_COLS, rec = w4_record_bytes(a.group);
     const int xg = a.xgroup ? a.xgroup : a.K, nxg = (a.K + xg - 1) / xg;
+    int last = -1;
+    bool nan = false;
     for (uint32_t asked = __ballot_sync(~0u, ask); asked; asked &= asked - 1) {
         const int who = __ffs(asked) - 1, row = __shfl_sync(~0u, m, who), r = __shfl_sync(~0u, n, who);
+        if (row != last) last = row, nan = nan_row(a, xtype, row);
+        if (nan) {
+            if (lane == who) v = __int_as_float(0x7fffffff);
+            continue;
+        }
         const uint8_t *w = static_cast<const uint8_t *>(a.w) + (int64_t)(r / W4_ROWS) * kb * rec;
         const int half = r % W4_ROWS / 8, low = r % 8;
         double sum = 0.;
@@ -187,14 +208,13 @@ __device__ __noinline__ float w4_plain(const W4Args &a, int xtype, bool ask, int
                 const double s = to_f32(reinterpret_cast<const bf16 *>(p + W4_CODE_BYTES)[j / a.group * W4_ROWS + r % W4_ROWS]);
                 const double xs = a.xscales[(int64_t)row * nxg + k0 / xg];
 #pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    if (k0 + c < a.K) {
-                        const int64_t at = row * a.ldx + k0 + c;
-                        const float x = xtype == TCB_I8 ? to_f32(static_cast<const int8_t *>(a.x)[at]) : to_f32(static_cast<const e4m3 *>(a.x)[at]);
-                        sum += x * xs * ((int)(codes >> 4 * (c / 2 + 4 * (c % 2)) & 15) - 8) * s;
-                    }
+                for (int c = 0; c < 8; ++c) {
+                    const int64_t at = row * a.ldx + min(k0 + c, a.K - 1);
+                    const float x = xtype == TCB_I8 ? to_f32(static_cast<const int8_t *>(a.x)[at]) : to_f32(static_cast<const e4m3 *>(a.x)[at]);
+                    if (k0 + c < a.K) sum += x * xs * ((int)(codes >> 4 * (c / 2 + 4 * (c % 2)) & 15) - 8) * s;
+                }
             }
-            if (__any_sync(~0u, sum != sum)) break;
+            if (__any_sync(~0u, sum != sum) || (__any_sync(~0u, sum > 1e300) && __any_sync(~0u, sum < -1e300))) break;  // NaN for good
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);

@@ -836,6 +836,34 @@ def test_gemv_w4_far_scales(lib, xtype, xgroup, xscale, wscale):
         within(y, want.to(torch.float32), mag * (K + K / 16 + 16) * 2 * U + want.abs() * U)
 
 
+@pytest.mark.parametrize("xgroup", [0, 32, 128])
+@pytest.mark.parametrize("xtype", [tb.I8, tb.E4M3])
+def test_gemv_w4_8_bit_rows_that_are_not_finite(lib, xtype, xgroup):
+    """Rows with a NaN code or scale are NaN; under an infinite scale each product has its sign (0 times it is NaN); other rows
+    stay as they are. The weights' zeros and signs differ from output to output."""
+    M, N, K = 12, 150, 2300
+    g, nxg = _gen(29), -(-K // xgroup) if xgroup else 1
+    codes = torch.randint(-8, 8, (N, K), device="cuda", generator=g, dtype=torch.int8)
+    codes[::3] = 1 + codes[::3].abs() % 7  # one sign, no zeros
+    codes[1::3, 2200:] = -3
+    w = torch.from_numpy(tb.w4_pack(codes.cpu().numpy(), 64, np.full((N, 36), 0.25, np.float32))).cuda()
+    x = torch.randint(1, 9, (M, K), device="cuda", generator=g).float()
+    x[5] *= torch.where(torch.rand(K, device="cuda", generator=g) < 0.5, -1.0, 1.0)
+    x[6, K - 1], x[9, 40:50] = 0, 0
+    x = x.to(TYPE[xtype])
+    xs = torch.full((M, nxg), 0.5, device="cuda")
+    xs[1], xs[2, -1], xs[9, 0] = float("nan"), float("nan"), float("inf")
+    xs[4, -1], xs[5], xs[6, -1], xs[7] = float("inf"), float("-inf"), float("inf"), float("-inf")
+    if xtype == tb.E4M3:
+        x.view(torch.uint8)[8, 1777], x.view(torch.uint8)[10] = 0x7f, 0xff
+    y = torch.zeros(M, N, device="cuda")
+    assert lib.tcb_op_gemv_w4(_p(x), K, xtype, _p(xs), xgroup, _p(w), 64, None, 0, None, 0, _p(y), N, tb.F32, M, N, K, _stream()) == 0
+    xd = x.double() * xs.double().repeat_interleave(xgroup or K, 1)[:, :K]
+    # the library's product in 64 bits may skip zeros: one sum of products per output
+    want = torch.stack([(row * codes.double() * 0.25).sum(1) for row in xd])
+    assert torch.equal(torch.nan_to_num(y.double(), 7, 8, 9), torch.nan_to_num(want, 7, 8, 9))  # whole quarters below 2^24: exact
+
+
 # ------------------------------------------------------------------ together
 def test_zero_rows_are_a_no_op(lib):
     x = torch.ones(64, device="cuda", dtype=torch.bfloat16)
