@@ -123,7 +123,10 @@ enum {
  * tcb_op_out128. Statistics are f32 and do not overflow for finite h. A NaN
  * makes its whole row NaN; an infinity makes its own v NaN and the row's other
  * v zero. A group with a NaN gets the scale NaN, int8 codes 0, e4m3 codes NaN.
- * A row's result does not depend on M or on the other rows.
+ * A row's result does not depend on M or on the other rows. Its last bits depend
+ * on how far its address in each tensor is behind a boundary of 8 elements, since
+ * that sets the order of the sum; a pitch that is a multiple of 8 gives all rows
+ * one order. h g is formed before the division, in f32: |h g| below 2^128.
  * sum may be x or res itself, and y of dtype may be x or sum (same pitch);
  * other overlaps are not allowed. */
 int tcb_op_rmsnorm(const void *x, int64_t ldx, const void *res, int64_t ldr, void *sum, int64_t lds, const float *g,

@@ -338,6 +338,19 @@ def test_rmsnorm_all_over_res(lib, D):
     check_rms(None, v, r, tb.BF16, 0, None)
 
 
+@pytest.mark.parametrize("D,ld,dtype", [(1337, 1341, tb.F16), (641, 641, tb.BF16), (99, 101, tb.F32)])
+def test_rmsnorm_same_row_elsewhere(lib, D, ld, dtype):
+    """Rows that are alike but start differently far behind a boundary are summed in other orders: twice the bound of one."""
+    g, M = _gen(30), 24
+    x = torch.zeros(M, ld, device="cuda", dtype=TYPE[dtype])
+    x[:, :D] = _randn(g, D).to(TYPE[dtype])
+    y, _, _ = run_rms(lib, x, None, None, D, dtype, dtype, 0, pad=ld - D)
+    one = y[:1].double()
+    within(y, one.expand(M, D).to(TYPE[dtype]), one.abs() * 2 * (HALF[dtype] * 2 + 64 * U) + TINY[dtype])
+    again, _, _ = run_rms(lib, x[:9], None, None, D, dtype, dtype, 0, pad=ld - D)
+    assert torch.equal(again, y[:9])
+
+
 # ------------------------------------------------------------------ rotary positions
 def rope_ref(x, pos, freq, mscale, rot, inter, inverse):
     """x: (M, heads, hd) f64; returns (out, magnitude of the two terms) in f64."""
