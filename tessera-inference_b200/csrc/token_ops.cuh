@@ -67,15 +67,4 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// round(q) to the code's type; |q| <= top up to rounding. A NaN q gives int8 0, e4m3 NaN.
-template <class T>
-__device__ __forceinline__ T to_code(float q) {
-    if constexpr (std::is_same_v<T, int8_t>) {
-        const float c = fminf(127.f, fmaxf(-127.f, rintf(q)));
-        return q != q ? (int8_t)0 : (int8_t)(int)c;
-    } else {
-        return e4m3(q);  // to nearest even, saturating
-    }
-}
-
 }  // namespace tcb
