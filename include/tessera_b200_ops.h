@@ -180,8 +180,9 @@ int tcb_rope_freqs(int rot, double base, int scaling, double factor, double span
  * TCB_F32. Products are exact and summed in f32 in an order that depends on
  * xtype, M, N, K, group, xgroup and the GPU's SMs only; the output is rounded
  * once. A code of 0 adds 0, whatever finite value it meets. The
- * weights are read once per 32 rows or so, so for hundreds of rows tcb_op_gemm
- * on bf16 weights is the faster call. M <= 2^18, N <= 2^24, K <= 65536. */
+ * weights are read once per 32 rows or so: tcb_op_gemm on bf16 weights is the
+ * faster call from some 64 rows on at 8,192 x 8,192 weights, from 128 at 2,560 x
+ * 1,280 and 1,920 x 640, from 192 at 2,560 x 2,560. M <= 2^18, N <= 2^24, K <= 65536. */
 int tcb_op_gemv_w4(const void *x, int64_t ldx, int xtype, const float *xscales, int xgroup, const void *w, int group,
                    const float *bias, int relu, const void *res, int64_t ldr, void *out, int64_t ldo, int otype, int M,
                    int N, int K, void *stream);

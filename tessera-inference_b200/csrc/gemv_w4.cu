@@ -24,10 +24,11 @@
 // the token rows of all K columns are too many for a block or the weight rows too
 // few for the SMs; the sums of the slices are joined over distributed shared memory.
 //
-// Measured (bf16 rows): 1 x 16,384 x 8,192 in 18.6 us, 3.7 TB/s of weights. Of that
-// 2 us are the launch and 4 the code's first run and the token rows, while only the
-// rings fill. 8 x 8,192 x 8,192 in 15.0 us, 32 x 8,192 x 8,192 in 30.4, 1 x 2,560 x
-// 1,280 in 4.8 us.
+// Measured (bf16 rows): 1 x 16,384 x 8,192 in 18.6 us, 3.7 TB/s of weights, with
+// scales of 32 in 22.7. Of that 2 us are the launch and 4 the code's first run and
+// the token rows, while only the rings fill; the codes' way to 16 bits keeps 63% of
+// the issue slots busy. 8 x 8,192 x 8,192 in 14.3 us, 32 x 8,192 x 8,192 in 29.6,
+// 1 x 2,560 x 1,280 in 4.4 us.
 #include <algorithm>
 #include <atomic>
 
@@ -39,7 +40,7 @@ namespace tcb {
 namespace {
 
 constexpr int W4_WARPS = 16, W4_THREADS = W4_WARPS * 32;
-constexpr int RING = 4;    // records in flight per warp; eight are faster by 2% at most on 46 sizes, and take room
+constexpr int RING = 4;    // records in flight per warp; eight are faster by 2% at most on 46 sizes and take the room of token rows
 constexpr int X_PAD = 32;  // 16-bit elements behind a staged token row: rows start 16 banks apart
 constexpr int SMEM_MAX = 227 * 1024;
 
@@ -364,7 +365,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
             float acc[NT][4] = {};
             uint32_t xo = r0 * W4_COLS * 2, so = my_xsc + r0 * (W4_COLS / SUB) * GROUP * 4;
             // two records' chains of products side by side, where the registers allow (one token on 16,384 x 8,192 with scales of
-            // 32: 23.4 us, one record at a time 25.1; with 32 tokens 36.7 and 36.0)
+            // 32: 23.0 us, one record at a time 24.8; 32 tokens on 8,192 x 8,192 31.1 and 30.0)
 #pragma unroll (NT == 1 ? 2 : 1)
             for (int r = 0; r < count; ++r) {
                 cp_async_wait<RING - 2>();

@@ -10,12 +10,12 @@
 //
 // Codes: with p = h g, v / s = p Q / max|p| whatever the row's norm is, so a code
 // comes from four roundings and differs from the definition's only where v / s is
-// that near the middle between two codes (41, 45 and 36 of 84 million e4m3 codes on
-// three inputs; f32 arithmetic in the definition's order: 62, 44 and 58).
+// that near the middle between two codes (28 to 44 of 84 million e4m3 codes on eight
+// inputs; f32 arithmetic in the definition's order: 33 to 66, more on each).
 //
 // Measured, bf16 rows: 524,288 x 640 with the residual to e4m3 with scales of 128
-// columns in 343 us (6.9 TB/s), to bf16 in 391 us (6.9 TB/s); 32,768 x 2,560 to e4m3
-// in 50 us (5.0 TB/s); 8,192 x 16,384 with the residual to int8 in 142 us (6.6 TB/s);
+// columns in 342 us (6.9 TB/s), to bf16 in 390 us (6.9 TB/s); 32,768 x 2,560 to e4m3
+// in 51 us (4.9 TB/s); 8,192 x 16,384 with the residual to int8 in 146 us (6.4 TB/s);
 // fp16 rows of 1,337 at a pitch of 1,341 to int8, 10,007 of them, in 34 us (2.8 TB/s,
 // bound by instructions: weights and edges come one by one).
 #pragma once
@@ -208,7 +208,8 @@ enum RmsMode { ALIGNED, EDGED, SINGLE, ALIGNED_ROW };
 
 // Threads of a block, and the registers of a thread, which bound the blocks on an SM: about what the packed row, and for
 // EDGED rows the row in f32, needs. Fewer spill, more leave HBM waiting (bf16 to e4m3, 524,288 x 640: 48 registers 396 us, 64
-// 422, 40 456; 32,768 x 2,560 with 64 threads a row: 80 registers 50 us, 96 54, 112 56).
+// 422, 40 456; 32,768 x 2,560 with 64 threads a row: 80 registers 50 us, 96 54, 112 56). Set on bf16 rows: f32 rows of six units
+// a thread, whose 9 blocks of two warps are five warps in a quarter of an SM, get 96 registers and spill.
 template <class T, int TEAM, int NU, RmsMode MODE>
 struct RmsShape {
     static constexpr int THREADS = TEAM <= 32 ? 128 : TEAM;

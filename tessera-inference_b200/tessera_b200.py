@@ -267,7 +267,7 @@ def w4_pack(w: np.ndarray, group: int, scales: np.ndarray | None = None) -> np.n
     lib = load_library()
     if scales is not None:
         w = np.asarray(w)
-        if not ((w >= -8) & (w <= 7) & (w == np.rint(w))).all():
+        if w.dtype != np.int8 and not ((w >= -8) & (w <= 7) & (w == np.rint(w))).all():  # tcb_w4_pack_codes checks int8
             raise ValueError("codes that are not whole numbers in -8..7")
     w = np.ascontiguousarray(w, np.float32 if scales is None else np.int8)
     N, K = w.shape
