@@ -11,9 +11,9 @@
 //
 // Products are exact, sums are f32; a group's sum is multiplied by its scale in f32. With the 2^-10 no group's sum leaves
 // f32's range, whatever bf16 values it has, and no product falls below its smallest step; the outputs are multiplied by 2^10.
-// Infinities and NaN among the activations take their course. Outputs of 8-bit x that
-// are not finite are computed again from the definition: a sum may leave f32's range before the scale that brings it back, and
-// an infinite scale meets each x there, not their sum.
+// Infinities and NaN among the activations take their course. Outputs of 8-bit x that are not finite are computed again from
+// the definition: a sum may leave f32's range before the scale that brings it back, and an infinite scale meets each x there,
+// not their sum.
 //
 // bf16 and fp16 token rows are staged as they are, 8-bit ones as fp16, which holds them exactly.
 //
@@ -27,8 +27,8 @@
 // Measured (bf16 rows): 1 x 16,384 x 8,192 in 18.6 us, 3.7 TB/s of weights, with
 // scales of 32 in 22.7. Of that 2 us are the launch and 4 the code's first run and
 // the token rows, while only the rings fill; the codes' way to 16 bits keeps 63% of
-// the issue slots busy. 8 x 8,192 x 8,192 in 14.3 us, 32 x 8,192 x 8,192 in 29.6,
-// 1 x 2,560 x 1,280 in 4.4 us.
+// the issue slots busy. 8 x 8,192 x 8,192 in 13.0 us (14.3 with scales of 64), 32 x
+// 8,192 x 8,192 in 29.6, 1 x 2,560 x 1,280 in 4.4 to 5.0 us.
 #include <algorithm>
 #include <atomic>
 
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
             float acc[NT][4] = {};
             uint32_t xo = r0 * W4_COLS * 2, so = my_xsc + r0 * (W4_COLS / SUB) * GROUP * 4;
             // two records' chains of products side by side, where the registers allow (one token on 16,384 x 8,192 with scales of
-            // 32: 23.0 us, one record at a time 24.8; 32 tokens on 8,192 x 8,192 31.1 and 30.0)
+            // 32: one record at a time takes 8% more; 32 tokens on 8,192 x 8,192: two take 3% more)
 #pragma unroll (NT == 1 ? 2 : 1)
             for (int r = 0; r < count; ++r) {
                 cp_async_wait<RING - 2>();
@@ -522,9 +522,10 @@ Fixed fixed_bytes(int group, int rows, int kb, int split, int sub, bool xg) {
 
 // The cheapest cut by a model in clock cycles: a record takes an SM 46 cycles at HBM's rate or 52 per 8 token rows (the codes'
 // way to 16 bits, the products, the fragments from shared memory), and a warp 500 and 200 per 8 token rows at least; a tile's
-// end 1,100, and 270 per slice that meets there, staging 2,000 and 9 bytes a cycle, a join 4,200. Fitted to every cut of 46
-// sizes of 1 to 64 token rows: what it takes is 0.7% slower than the best in the mean, 5.4% at most. Sizes only: the cut sets
-// the order of the sums, and pointers' alignment shall not.
+// end 1,100, and 270 per slice that meets there, staging 2,000 and 17 bytes in two, a join 4,200. Fitted to every cut of 46
+// sizes of 1 to 64 token rows: what it takes is 0.6% slower than the best in the mean, 5% at most (1.2% and 5% on 38
+// sizes of one to four rows that it was not fitted to). Sizes only: the cut sets the order of the sums, and pointers' alignment
+// shall not.
 // Returns its cost, or INT64_MAX where nothing fits.
 int64_t best_cut(const W4Args &a, int mt, int sub, bool xg, int split, int blocks, W4Cut &out, int &bytes) {
     const int kb = (a.K + W4_COLS - 1) / W4_COLS, tiles = (a.N + W4_ROWS - 1) / W4_ROWS, nt = (out.rows + 7) / 8;
@@ -543,7 +544,7 @@ int64_t best_cut(const W4Args &a, int mt, int sub, bool xg, int split, int block
         }
         const int64_t count = ((kb + split - 1) / split + wk - 1) / wk;
         int64_t cost = std::max((int64_t)each * ((kb + split - 1) / split) * std::max(46, 52 * nt), batches * steps * count * (500 + 200 * nt));
-        cost += 2000 + f.x / 9 + (int64_t)batches * steps * (1100 + (wk > 1 ? 270 * wk : 0));
+        cost += 2000 + f.x * 2 / 17 + (int64_t)batches * steps * (1100 + (wk > 1 ? 270 * wk : 0));
         if (split > 1) cost += batches * 4200;
         if (cost >= best) continue;
         best = cost;
